@@ -15,7 +15,7 @@
  *   - `stream` is a hipStream_t passed as void* (NULL = the default stream).
  *     Calls with host pointers are synchronous. Calls with device pointers are
  *     stream-ordered; on an index with fp32 rows only (storage 0) they return
- *     without synchronising. With a bf16 copy (storage 1 or 2) ipx_search /
+ *     without synchronising. With a bf16 copy or 4-bit rows (storage 1, 2, 3) ipx_search /
  *     ipx_search_aspect / ipx_search_pooled read back one flag word per query
  *     after the rescoring pass (which queries the margin rule sends to a repeat
  *     pass) and so synchronise the stream once per pass before they return;
@@ -156,6 +156,42 @@ int ipx_search_pooled(ipx_index* idx, const float* hidden, int64_t seq_len, cons
                       int begin_id, int64_t nq, int k, float* out_D, int64_t* out_I, float* out_att,
                       int on_device, void* stream);
 
+/* ---- rows in microscaled 4-bit floating point (mx4; no counterpart in the reference) ----------------------------
+ * 32 consecutive elements of a row share the scale 2^s, s = max(floor(log2(largest magnitude)) - 2, -127), held as the
+ * byte s + 127; an element is the E2M1 code (+-{0, 0.5, 1, 1.5, 2, 3, 4, 6}, code = sign << 3 | index) nearest to
+ * element / 2^s, ties to the even code, magnitudes beyond 6 to 6. A block with a NaN or an infinity has the scale byte
+ * 255 and stands for 32 NaNs. The last block of a row may be short. 17 bytes per 32 elements.
+ * External form, nb = ceil(d / 32) blocks per row: codes [n][nb][16] bytes, element 2i of a block in the low nibble of
+ * byte i; scales [n][nb] bytes. (OCP microscaling formats, MXFP4.)
+ *
+ * ipx_mx4_quantize: rows [n, d] of `dtype`, `stride` elements apart (>= d) -> codes (a multiple of 4 bytes), scales.
+ * ipx_mx4_dequantize: back to values [n, d] of `dtype`; exact in fp32 and bf16, rounded to nearest even in f16.
+ * Neither allocates nor synchronises with on_device != 0. `device`: the GPU of the pointers, or the one to use. */
+int ipx_mx4_quantize(const void* rows, int64_t n, int d, int64_t stride, int dtype, uint8_t* codes, uint8_t* scales,
+                     int on_device, int device, void* stream);
+int ipx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n, int d, void* out, int dtype,
+                       int on_device, int device, void* stream);
+
+/* Appends rows that are in mx4 already (storage 3 only; ipx_add quantises rows on the way in). Codes behind element d
+ * of a row's last block are ignored. */
+int ipx_add_mx4(ipx_index* idx, const uint8_t* codes, const uint8_t* scales, int64_t n, int on_device, void* stream);
+
+/* out[i][j] = <q_i, row row0 + j of the index>, fp32 [nq, n], storage 3 only. q: [nq, d] of q_dtype, taken to within 2^-20
+ * of the largest magnitude of each block of 32 elements (in practice 2^-24), products and sums in fp32; a query with a
+ * NaN or an infinity is multiplied element by element. ipx_scores_mx4: queries in mx4, products exact.
+ * With on_device != 0 stream-ordered; the first call of a size allocates the index's query buffers. */
+int ipx_scores(ipx_index* idx, const void* q, int q_dtype, int64_t nq, int64_t row0, int64_t n, float* out,
+               int on_device, void* stream);
+int ipx_scores_mx4(ipx_index* idx, const uint8_t* q_codes, const uint8_t* q_scales, int64_t nq, int64_t row0, int64_t n,
+                   float* out, int on_device, void* stream);
+
+/* out[i] = scale[i] * (the stored row with id ids[i]), [n, d] of `dtype`; any storage (the values the index keeps: fp32
+ * rows, rounded bf16 rows, mx4 values). scale: fp32 [n], NULL = 1. Ids as a search returns them (id_base included); the
+ * empty slot -1 gives a row of zeros. Any other id outside the index is IPX_ERR_ARG with host pointers; with device
+ * pointers its row is zeros and the next ipx_check reports it. Neither allocates nor synchronises with on_device != 0. */
+int ipx_lookup(ipx_index* idx, const int64_t* ids, int64_t n, const float* scale, void* out, int dtype, int on_device,
+               void* stream);
+
 /* Replaces faiss.ResultHeap(nq,k).add_result(-D_s, I_s) for s in shards; finalize()
  *                                                      reducer.py:15-18
  * D: fp32 [S, nq, k_in], I: int64 [S, nq, k_in] (one block per shard, ids already
@@ -174,7 +210,7 @@ int ipx_merge_topk_packed(const void* packed, int S, int64_t nq, int k_in, int k
                           float* out_D, int64_t* out_I, int device, void* stream);
 
 /* Index options and tuning knobs. Search RESULTS never depend on any of them, with one
- * documented exception: storage 2 defines the exact score on the bf16-rounded rows.
+ * documented exception: storage 2 (3) defines the exact score on the bf16-rounded (4-bit) rows.
  *   "storage"    : what the index keeps of the added rows; only while the index is empty.
  *                  0 (default) fp32 rows, fp32 MFMA scan.
  *                  1 fp32 rows + a bf16 copy: bf16 MFMA scan for candidates, exact fp32
@@ -183,6 +219,9 @@ int ipx_merge_topk_packed(const void* packed, int S, int64_t nq, int k_in, int k
  *                  2 bf16 rows only (rows given as bf16 are kept exactly, fp32 / f16 rows are
  *                    rounded to nearest even): bf16 scan, then exact fp32 scores of
  *                    <fp32 query, stored bf16 row>; half the HBM of storage 0; k <= 8192.
+ *                  3 mx4 rows only (see ipx_mx4_quantize): 4-bit scan, then exact fp32 scores of <fp32 query, stored
+ *                    4-bit values> — bit for bit what storage 2 returns for rows given as those values; 17 bytes per
+ *                    32 elements, 0.13 of storage 0; k <= 2048.
  *                  Queries whose candidate list cannot be proven sufficient (more near-ties than the longest
  *                  list holds: thousands of duplicate rows, a degenerate embedding) are repeated — storage 1: on
  *                  the fp32 scan; storage 2: by an exact pass over every stored row, slow but never an error.

@@ -16,6 +16,7 @@ SYMBOLS = [
     "ipx_last_error", "ipx_version", "ipx_device_count", "ipx_create", "ipx_destroy", "ipx_dim",
     "ipx_ntotal", "ipx_reserve", "ipx_set_id_base", "ipx_add", "ipx_search", "ipx_search_noalloc", "ipx_search_aspect", "ipx_search_pooled", "ipx_pool", "ipx_add_pooled",
     "ipx_merge_topk", "ipx_merge_topk_packed", "ipx_packed_block_bytes", "ipx_set_param", "ipx_read_trace", "ipx_check", "ipx_set_timing", "ipx_last_timing", "ipx_last_geometry",
+    "ipx_mx4_quantize", "ipx_mx4_dequantize", "ipx_add_mx4", "ipx_scores", "ipx_scores_mx4", "ipx_lookup",
     "ipx_last_bf16_stats", "ipx_outlier_rows", "ipx_last_exact_queries",
     "ipx_write_ranking", "ipx_write_ranking_lookup", "ipx_format_score",
 ]
@@ -68,6 +69,12 @@ def lib():
     L.ipx_search_pooled.argtypes = [vp, f32p, i64, f32p, f32p, i32, i32, i64, i32, f32p, i64p, f32p, i32, vp]
     L.ipx_pool.argtypes = [vp, f32p, i64, f32p, f32p, i32, i32, i64, f32p, f32p, i32, vp]
     L.ipx_add_pooled.argtypes = [vp, f32p, i64, f32p, f32p, i32, i32, i64, i32, vp]
+    L.ipx_mx4_quantize.argtypes = [vp, i64, i32, i64, i32, vp, vp, i32, i32, vp]
+    L.ipx_mx4_dequantize.argtypes = [vp, vp, i64, i32, vp, i32, i32, i32, vp]
+    L.ipx_add_mx4.argtypes = [vp, vp, vp, i64, i32, vp]
+    L.ipx_scores.argtypes = [vp, vp, i32, i64, i64, i64, vp, i32, vp]
+    L.ipx_scores_mx4.argtypes = [vp, vp, vp, i64, i64, i64, vp, i32, vp]
+    L.ipx_lookup.argtypes = [vp, i64p, i64, f32p, vp, i32, i32, vp]
     L.ipx_merge_topk.argtypes = [f32p, i64p, i32, i64, i32, i32, f32p, i64p, i32, i32, vp]
     L.ipx_merge_topk_packed.argtypes = [vp, i32, i64, i32, i32, f32p, i64p, i32, vp]
     L.ipx_packed_block_bytes.argtypes = [i64, i32]

@@ -8,6 +8,7 @@
 #include "ipx_bf16_kernels.h"
 #include "ipx_f32_small_kernels.h"
 #include "ipx_bf16_w16_kernels.h"
+#include "ipx_mx4_kernels.h"
 // The default library ships ONE large-batch bf16 scan (the 16-wave kernel, 2-deep ring: 16x16x32 MFMA with one query
 // part, 32x32x16 with hi + lo parts). The kernels and kernel variants that were built to find it and never won — the
 // 8-wave tile, the ping-pong and direct-corpus-operand kernels, the 384 x 256 tile on 12 waves, deeper rings, issue
@@ -20,6 +21,7 @@
 #include "ipx_bf16_w12_kernels.h"
 #endif
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -141,6 +143,9 @@ int next_pow2(int x) {
 
 }  // namespace
 
+// word of ipx_index::err that ipx_lookup sets (word 0 belongs to the searches)
+constexpr int LOOKUP_ERR = 16;
+
 struct ipx_index {
     int d = 0, nks = 0, device = 0;
     int num_cus = 0;         // multiProcessorCount of `device`, read once at create
@@ -151,11 +156,18 @@ struct ipx_index {
     float* Xp = nullptr;     // packed fp32 corpus (storage 0, 1)
     // storage: 0 = fp32 rows, fp32 scan; 1 = fp32 rows + a bf16 copy: bf16 scan, fp32 rescoring;
     //          2 = bf16 rows only (rows given as bf16, or rounded on add): bf16 scan, exact
-    //              rescoring of the stored bf16 values against the fp32 query
+    //              rescoring of the stored bf16 values against the fp32 query;
+    //          3 = mx4 rows only (ipx_mx4_kernels.h): scaled-MFMA scan, exact rescoring of the 4-bit values
     int storage = 0;
+    bool lookups = false;    // ipx_lookup has run on device ids: ipx_check reads its error word too
     int nks_h = 0;           // K-stages of 32 bf16
     int64_t cap_tiles_h = 0; // tiles of 256 rows the bf16 buffer holds
     uint16_t* Xh = nullptr;  // packed bf16 corpus (storage 1, 2)
+    int nks_x = 0, nkq_x = 0;      // mx4: K-sets of 64 elements, quads of K-sets
+    int64_t cap_groups_x = 0;      // groups of 32 rows the mx4 buffers hold (always whole tiles)
+    uint8_t* Xx = nullptr;         // mx4 codes (storage 3)
+    uint8_t* Xxs = nullptr;        // mx4 scales
+    DevBuf mxq, mxs;               // a pass's floors and query norms; the sample's scores
     DevBuf Qp, cand, partD, partI, err, stageIn, stageQ, stageW, outD, outI, trace, pub;
     DevBuf outl, olist, sideD, sideI;   // outlier rows of an index with fp32 rows + bf16 copy (row_sumsq_max_kernel)
     bool outl_thr_set = false;
@@ -204,6 +216,8 @@ struct ipx_index {
     bool force_f32_scan = false;   // storage 1: use the fp32 scan although a bf16 copy exists
     size_t tile_bytes() const { return (size_t)nks * ipx::STAGE_A_BYTES; }
     size_t tile_bytes_h() const { return (size_t)nks_h * ipx::HSTAGE_A; }
+    size_t group_bytes_x() const { return (size_t)nks_x * ipx::MX_SET_BYTES; }
+    size_t group_scales_x() const { return (size_t)nkq_x * 256; }
 };
 
 namespace {
@@ -264,6 +278,78 @@ int grow_corpus_h(ipx_index* ix, int64_t need_tiles, hipStream_t st) {
     return 0;
 }
 
+// Room for need_groups groups of 32 mx4 rows, codes and scales; rows not yet added read as zeros.
+int grow_corpus_x(ipx_index* ix, int64_t need_groups, hipStream_t st) {
+    need_groups = (need_groups + 7) / 8 * 8;
+    if (need_groups <= ix->cap_groups_x) return 0;
+    int64_t want = std::max(need_groups, (ix->cap_groups_x + ix->cap_groups_x / 2 + 7) / 8 * 8);
+    const size_t gb = ix->group_bytes_x(), gs = ix->group_scales_x();
+    uint8_t *nb = nullptr, *ns = nullptr;
+    hipError_t e = hipMalloc((void**)&nb, (size_t)want * gb);
+    if (e != hipSuccess && want > need_groups) {
+        want = need_groups;
+        e = hipMalloc((void**)&nb, (size_t)want * gb);
+    }
+    if (e == hipSuccess) e = hipMalloc((void**)&ns, (size_t)want * gs);
+    if (e != hipSuccess) {
+        if (nb) (void)hipFree(nb);
+        return fail(IPX_ERR_NOMEM, std::string("hipMalloc(mx4 corpus): ") + hipGetErrorString(e));
+    }
+    const size_t old = (size_t)ix->cap_groups_x;
+    if (old) e = hipMemcpyAsync(nb, ix->Xx, old * gb, hipMemcpyDeviceToDevice, st);
+    if (e == hipSuccess && old) e = hipMemcpyAsync(ns, ix->Xxs, old * gs, hipMemcpyDeviceToDevice, st);
+    if (e == hipSuccess) e = hipMemsetAsync(nb + old * gb, 0, ((size_t)want - old) * gb, st);
+    if (e == hipSuccess) e = hipMemsetAsync(ns + old * gs, 0, ((size_t)want - old) * gs, st);
+    if (e == hipSuccess && old) e = hipStreamSynchronize(st);
+    if (e != hipSuccess) {
+        (void)hipFree(nb);
+        (void)hipFree(ns);
+        return fail(IPX_ERR_HIP, std::string("grow mx4 corpus: ") + hipGetErrorString(e));
+    }
+    if (ix->Xx) (void)hipFree(ix->Xx);
+    if (ix->Xxs) (void)hipFree(ix->Xxs);
+    ix->Xx = nb;
+    ix->Xxs = ns;
+    ix->cap_groups_x = want;
+    return 0;
+}
+
+// Division of a thread number by `by` on the device (div_by in ipx_mx4_kernels.h).
+uint64_t magic_of(uint64_t by) { return by <= 1 ? 0 : ~0ull / by + 1; }
+// A launch numbers its threads with 32 bits: rows per launch when a row takes `per_row` of them.
+int64_t rows_per_launch(int64_t per_row) { return std::max<int64_t>(1, (int64_t)(1ll << 31) / per_row); }
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Rows (device, `stride` elements apart) -> mx4: codes / scales in the external form, or rows row0.. of index ix.
+int launch_mx4_quantize(const void* rows, int dtype, int64_t n, int d, int64_t stride, uint8_t* codes, uint8_t* scales,
+                        ipx_index* ix, int64_t row0, hipStream_t st) {
+    const int nb = (d + 31) / 32, np = nb * 4;
+    const size_t el = dtype == IPX_F32 ? 4 : 2;
+    const bool wide = aligned16(rows) && stride * el % 16 == 0;
+    const int64_t slice = rows_per_launch(np);
+    for (int64_t r0 = 0; r0 < n; r0 += slice) {
+        const uint32_t total = (uint32_t)(std::min(slice, n - r0) * np);
+        const void* src = (const char*)rows + (size_t)r0 * stride * el;
+        const dim3 grid((total + 255) / 256), block(256);
+        if (ix)
+            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<true>, grid, block, 0, st, src, dtype, stride, total, magic_of(np), np, d,
+                               wide, ix->Xx, ix->Xxs, row0 + r0, ix->nks_x, ix->nkq_x);
+        else
+            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<false>, grid, block, 0, st, src, dtype, stride, total, magic_of(np), np, d,
+                               wide, codes + (size_t)r0 * nb * 16, scales + (size_t)r0 * nb, (int64_t)0, 0, 0);
+        IPX_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+int launch_mx4_norms(ipx_index* ix, int64_t row0, int64_t n, hipStream_t st) {
+    const int blocks = (int)std::min<int64_t>((n / 32 + 2 + 3) / 4, 2048);
+    hipLaunchKernelGGL(ipx::mx4_norm_max_kernel, dim3(blocks), dim3(256), 0, st, ix->Xx, ix->Xxs, row0, n, ix->nks_x, ix->nkq_x,
+                       (uint32_t*)ix->maxsq.p);
+    IPX_HIP(hipGetLastError());
+    return 0;
+}
+
 int launch_pack_bf16(const void* src, int dtype, int64_t n, int64_t n_pad, int d, uint16_t* dst, int64_t row0,
                      int rows_per_tile, int nks_h, int parts, hipStream_t st, int swz = 0, void* zero = nullptr,
                      size_t zero_bytes = 0) {
@@ -291,6 +377,10 @@ int launch_pack(const void* src, int dtype, int64_t n, int64_t n_pad, int d, flo
 
 // one slice of rows, already on the device: every copy this index keeps + the norm bound
 int add_device_rows(ipx_index* ix, const void* rows, int dtype, int64_t m, int64_t row0, hipStream_t st) {
+    if (ix->storage == 3) {
+        if (int rc = launch_mx4_quantize(rows, dtype, m, ix->d, ix->d, nullptr, nullptr, ix, row0, st)) return rc;
+        return launch_mx4_norms(ix, row0, m, st);
+    }
     if (ix->storage != 2)
         if (int rc = launch_pack(rows, dtype, m, m, ix->d, ix->Xp, row0, ipx::BD, ix->nks, nullptr, 0, 0, st)) return rc;
     if (ix->storage != 0) {
@@ -317,6 +407,14 @@ int add_device_rows(ipx_index* ix, const void* rows, int dtype, int64_t m, int64
 
 // room for n rows in every copy this index keeps
 int grow_storage(ipx_index* ix, int64_t n, hipStream_t st) {
+    if (ix->storage == 3) {
+        if (int rc = grow_corpus_x(ix, (n + ipx::MX_GROUP - 1) / ipx::MX_GROUP, st)) return rc;
+        if (!ix->maxsq.p) {
+            if (int rc = ix->maxsq.ensure(256)) return rc;
+            IPX_HIP(hipMemsetAsync(ix->maxsq.p, 0, 256, st));
+        }
+        return 0;
+    }
     if (ix->storage != 2)
         if (int rc = grow_corpus(ix, (n + ipx::BD - 1) / ipx::BD, st)) return rc;
     if (ix->storage != 0) {
@@ -338,16 +436,20 @@ int dtype_size(int dtype) { return dtype == IPX_F32 ? 4 : 2; }
 struct Geometry { int nqb, ntiles, S, R, G, cap; };
 
 // Deep lists: the splits' unsorted lists of every query (ScanParams::deepK / deepN) -> sorted top k_out (dD / dI).
-int launch_deep_finish(ipx_index* ix, int S, int k_list, int k_out, int64_t nq, float* dD, int64_t* dI, hipStream_t st) {
+int launch_lists_finish(ipx_index* ix, const uint64_t* keys, const int* counts, int S, int k_list, int k_out, int64_t nq, float* dD,
+                        int64_t* dI, hipStream_t st) {
     const int64_t total = (int64_t)S * k_list;
     const int P_max = (int)std::min<int64_t>(ipx::DEEP_LDS_KEYS, next_pow2((int)std::min<int64_t>(total, ipx::DEEP_LDS_KEYS)));
     const int lds = std::max(P_max, 2) * 8 + (S + 1) * 4 + 256 * 4;
     if (lds > 64 * 1024)
         IPX_HIP(hipFuncSetAttribute((const void*)ipx::deep_finish_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    hipLaunchKernelGGL(ipx::deep_finish_kernel, dim3((unsigned)nq), dim3(1024), lds, st, (const uint64_t*)ix->deepK.p,
-                       (const int*)ix->deepN.p, S, k_list, k_out, std::max(P_max, 2), ix->id_base, dD, dI);
+    hipLaunchKernelGGL(ipx::deep_finish_kernel, dim3((unsigned)nq), dim3(1024), lds, st, keys, counts, S, k_list, k_out, std::max(P_max, 2), ix->id_base, dD, dI);
     IPX_HIP(hipGetLastError());
     return 0;
+}
+
+int launch_deep_finish(ipx_index* ix, int S, int k_list, int k_out, int64_t nq, float* dD, int64_t* dI, hipStream_t st) {
+    return launch_lists_finish(ix, (const uint64_t*)ix->deepK.p, (const int*)ix->deepN.p, S, k_list, k_out, nq, dD, dI, st);
 }
 
 // ---- fp32 scan of a small batch (scan_f32_small_kernel: 32 or 64 queries per workgroup, two workgroups per CU):
@@ -680,14 +782,42 @@ int scan_f32_deep(ipx_index* ix, const float* dq, const float* dw, int A, int lo
 
 // rescore_kernel over `nblocks` lists: 16 waves per list for the few lists of a small batch (latency), 4 otherwise.
 int launch_rescore(const ipx::RescoreParams& rp, int64_t nblocks, hipStream_t st) {
-    const int fixed = ((rp.nks * (rp.x_is_bf16 ? 32 : 16) * 4 + 15) & ~15) + rp.P * 8 + (rp.P <= ipx::RS_RANK_SORT ? rp.P * 8 : 0);
+    const int dpad = rp.xfmt == 2 ? (rp.nks + 1) / 2 * 128 : rp.nks * (rp.xfmt ? 32 : 16);
+    const int fixed = ((dpad * 4 + 15) & ~15) + rp.P * 8 + (rp.P <= ipx::RS_RANK_SORT ? rp.P * 8 : 0);
     const int per_wave = ipx::RS_KB * 16 * ipx::RS_ROW;
     const int nw = (nblocks <= 128 && fixed + 16 * per_wave <= 160 * 1024) ? 16 : 4;
     const int rlds = fixed + nw * per_wave;
-    void (*kern)(const ipx::RescoreParams) = nw == 16 ? ipx::rescore_kernel<16> : ipx::rescore_kernel<4>;
+    void (*kern)(const ipx::RescoreParams) = rp.xfmt == 2 ? (nw == 16 ? ipx::rescore_kernel<16, true> : ipx::rescore_kernel<4, true>)
+                                                          : (nw == 16 ? ipx::rescore_kernel<16> : ipx::rescore_kernel<4>);
     if (int rc = ensure_dynamic_lds((const void*)kern, rlds)) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)nblocks), dim3(nw * 64), rlds, st, rp);
     IPX_HIP(hipGetLastError());
+    return 0;
+}
+
+// The rows the exact scores of this index are defined on.
+void rescore_rows(const ipx_index* ix, ipx::RescoreParams& rp) {
+    rp.xfmt = ix->storage == 3 ? 2 : ix->storage == 2 ? 1 : 0;
+    rp.X = rp.xfmt == 2 ? (const void*)ix->Xx : rp.xfmt ? (const void*)ix->Xh : (const void*)ix->Xp;
+    rp.nks = rp.xfmt == 2 ? ix->nks_x : rp.xfmt ? ix->nks_h : ix->nks;
+    if (rp.xfmt == 2) {
+        rp.Xs = ix->Xxs;
+        rp.nkq = ix->nkq_x;
+        rp.qinfo = (const float*)ix->mxq.p;      // (mx4_pass: the first block of this buffer)
+    }
+}
+
+// Room for a pass's nq flags + 2 words in pinned host memory (rescore_kernel writes them there: one wait, no copy).
+int ensure_hflags(ipx_index* ix, int64_t nq, hipStream_t st) {
+    if (ix->hflags_n >= (size_t)nq + 2) return 0;
+    IPX_HIP(hipStreamSynchronize(st));          // (an earlier pass's kernel may still write the old block)
+    if (ix->hflags) (void)hipHostFree(ix->hflags);
+    ix->hflags = nullptr;
+    ix->hflags_n = 0;
+    const size_t want = std::max<size_t>((size_t)nq + 2, 4096);
+    hipError_t e = hipHostMalloc((void**)&ix->hflags, want * sizeof(int), hipHostMallocDefault);
+    if (e != hipSuccess) { ix->hflags = nullptr; return fail(IPX_ERR_NOMEM, std::string("hipHostMalloc: ") + hipGetErrorString(e)); }
+    ix->hflags_n = want;
     return 0;
 }
 
@@ -905,25 +1035,14 @@ int bf16_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, int qpa
 
     // the pass's flags (which queries failed the margin check; behind them the scan's error word and the outlier count)
     // are written by the rescoring kernel straight into pinned host memory: one wait, no copy
-    if (ix->hflags_n < (size_t)nq + 2) {
-        IPX_HIP(hipStreamSynchronize(st));          // (an earlier pass's kernel may still write the old block)
-        if (ix->hflags) (void)hipHostFree(ix->hflags);
-        ix->hflags = nullptr;
-        ix->hflags_n = 0;
-        const size_t want = std::max<size_t>((size_t)nq + 2, 4096);
-        hipError_t e = hipHostMalloc((void**)&ix->hflags, want * sizeof(int), hipHostMallocDefault);
-        if (e != hipSuccess) { ix->hflags = nullptr; return fail(IPX_ERR_NOMEM, std::string("hipHostMalloc: ") + hipGetErrorString(e)); }
-        ix->hflags_n = want;
-    }
+    if (int rc = ensure_hflags(ix, nq, st)) return rc;
     ipx::RescoreParams rp;
     rp.candD = (const float*)ix->candD.p;
     rp.candI = (const int64_t*)ix->candI.p;
     rp.todo = pool_todo;
     rp.q = qf;
     rp.qmap = nullptr;
-    rp.x_is_bf16 = ix->storage == 2;
-    rp.X = rp.x_is_bf16 ? (const void*)ix->Xh : (const void*)ix->Xp;
-    rp.nks = rp.x_is_bf16 ? ix->nks_h : ix->nks;
+    rescore_rows(ix, rp);
     rp.maxsq = (const uint32_t*)ix->maxsq.p;
     rp.outD = dD;
     rp.outI = dI;
@@ -1018,9 +1137,7 @@ int exact_rows_path(ipx_index* ix, const float* qf, const std::vector<int>& sel,
     rp.candI = (const int64_t*)lI.p;
     rp.q = qf;
     rp.qmap = (const int*)ix->sel.p;
-    rp.x_is_bf16 = ix->storage == 2;
-    rp.X = rp.x_is_bf16 ? (const void*)ix->Xh : (const void*)ix->Xp;
-    rp.nks = rp.x_is_bf16 ? ix->nks_h : ix->nks;
+    rescore_rows(ix, rp);
     rp.maxsq = (const uint32_t*)ix->maxsq.p;
     rp.outD = (float*)ix->partD.p;
     rp.outI = (int64_t*)ix->partI.p;
@@ -1077,7 +1194,7 @@ int merge_outlier_rows(ipx_index* ix, const float* qf, int64_t nq, int k, float*
     rp.q = qf;
     rp.qmap = nullptr;
     rp.shared_list = 1;
-    rp.x_is_bf16 = 0;
+    rp.xfmt = 0;
     rp.X = (const void*)ix->Xp;
     rp.nks = ix->nks;
     rp.maxsq = (const uint32_t*)ix->maxsq.p;
@@ -1108,6 +1225,17 @@ int merge_outlier_rows(ipx_index* ix, const float* qf, int64_t nq, int k, float*
     return 0;
 }
 
+// aspect embeddings + weights -> row-major fp32 queries in ix->qfused
+int fuse_queries(ipx_index* ix, const float* dq, const float* dw, int A, int logits, int64_t nq, hipStream_t st, const float** out) {
+    const int64_t total = nq * (int64_t)ix->d;
+    if (int rc = ix->qfused.ensure((size_t)total * sizeof(float))) return rc;
+    hipLaunchKernelGGL(ipx::fuse_aspect_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, dq, dw, A, logits, nq,
+                       ix->d, (float*)ix->qfused.p);
+    IPX_HIP(hipGetLastError());
+    *out = (const float*)ix->qfused.p;
+    return 0;
+}
+
 // Longest candidate list of a bf16 pass (the API's single-pass depth IPX_MAX_K is about result lists; candidate
 // lists may be longer: their queues live in HBM, a selection takes 4 bytes of LDS per queue slot, the final sort 8).
 constexpr int MAX_KC = 4096;
@@ -1117,7 +1245,6 @@ constexpr int MAX_KC = 4096;
 // the bf16 rows (storage 2).
 int scan_bf16_path(ipx_index* ix, const float* dq, const float* dw, int A, int logits, int64_t nq, int k,
                    float* dD, int64_t* dI, hipStream_t st) {
-    const int d = ix->d;
     // One bf16 part per query and 5k candidates (2k when only the query is rounded) while that
     // list stays short; deeper searches split the query into hi + lo parts — the margin then only
     // carries the rows' rounding (none in storage 2) — and keep 2k (1.25k) candidates.
@@ -1171,14 +1298,8 @@ int scan_bf16_path(ipx_index* ix, const float* dq, const float* dw, int A, int l
     kc = std::min(std::max(kc, k), kc_max);
 
     const float* qf = dq;
-    if (A > 0) {   // the fused fp32 query is needed row-major for the rescoring
-        if (int rc = ix->qfused.ensure((size_t)nq * d * sizeof(float))) return rc;
-        const int64_t total = nq * (int64_t)d;
-        hipLaunchKernelGGL(ipx::fuse_aspect_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, dq, dw, A,
-                           logits, nq, d, (float*)ix->qfused.p);
-        IPX_HIP(hipGetLastError());
-        qf = (const float*)ix->qfused.p;
-    }
+    if (A > 0)     // the fused fp32 query is needed row-major for the rescoring
+        if (int rc = fuse_queries(ix, dq, dw, A, logits, nq, st, &qf)) return rc;
     // flagged: a longer list may do; hard: no bf16 list can (they skip the repeat pass)
     std::vector<int> flagged, hard;
     if (int rc = bf16_pass(ix, qf, nq, k, kc, qparts, dD, dI, st, true, flagged, hard)) return rc;
@@ -1219,6 +1340,264 @@ int scan_bf16_path(ipx_index* ix, const float* dq, const float* dw, int A, int l
     return redo_queries(ix, qf, flagged, k, dD, dI, st, [&](const float* q2, int64_t n2, float* D2, int64_t* I2) {
         return scan_f32_path(ix, q2, nullptr, 0, 0, n2, k, D2, I2, st, false);
     });
+}
+
+// ---- mx4 rows (storage 3) -------------------------------------------------------------------------------------
+constexpr int MX_PARTS_SEARCH = 2;       // E2M3 parts per query in the scan: what they leave out enters the margin rule
+constexpr int MX_PARTS_SCORES = 5;       // ... in ipx_scores: as exact as fp32
+constexpr int MX_MAX_K = IPX_MAX_K;      // deepest list of a search
+constexpr int MX_SLICE = 4096;           // queries per pass of a search (bounds the workspace)
+
+// How a product runs: queries per workgroup, quads of the query block in LDS at a time, splits of the corpus.
+struct MxGeom { int cg, qc, nqb, S, lds; int64_t rounds; };
+MxGeom mx4_geometry(const ipx_index* ix, int64_t nq, int quad_bytes_per_cg, int64_t ntiles) {
+    MxGeom g;
+    const int room = 160 * 1024 - 1024, extra = 128;         // extra: hit counters, 4 bytes per query
+    // the largest block (more queries per row operand) whose queries stay in LDS; when not even 32 queries fit (long
+    // vectors), the quads go through LDS in turn
+    g.cg = nq <= 32 ? 1 : nq <= 64 ? 2 : 4;
+    const int want = g.cg;
+    while (g.cg > 1 && ix->nkq_x * quad_bytes_per_cg * g.cg + extra * g.cg > room) g.cg /= 2;
+    if (ix->nkq_x * quad_bytes_per_cg * g.cg + extra * g.cg > room) {
+        g.cg = want;
+        while (quad_bytes_per_cg * g.cg + extra * g.cg > room) g.cg /= 2;
+    }
+    g.qc = std::min(ix->nkq_x, (room - extra * g.cg) / (quad_bytes_per_cg * g.cg));
+    g.lds = g.qc * quad_bytes_per_cg * g.cg + extra * g.cg;
+    const int per_cu = g.lds <= 80 * 1024 - 512 ? 2 : 1;
+    g.nqb = (int)((nq + 32 * g.cg - 1) / (32 * g.cg));
+    const int64_t most = std::max<int64_t>(1, (ntiles + 7) / 8);       // 8 waves, a tile each
+    g.S = (int)std::min<int64_t>(std::max(1, per_cu * ix->num_cus / g.nqb), most);
+    g.rounds = (ntiles + (int64_t)g.S * 8 - 1) / ((int64_t)g.S * 8);
+    return g;
+}
+
+template <int PARTS, int FMT, int MODE>
+int launch_mx4_product(const MxGeom& g, ipx::MxParams p, hipStream_t st) {
+    p.S = g.S;
+    p.qc = g.qc;
+    void (*kern)(const ipx::MxParams) = g.cg == 1 ? ipx::mx4_product_kernel<1, PARTS, FMT, MODE>
+                                        : g.cg == 2 ? ipx::mx4_product_kernel<2, PARTS, FMT, MODE>
+                                                    : ipx::mx4_product_kernel<4, PARTS, FMT, MODE>;
+    if (int rc = ensure_dynamic_lds((const void*)kern, std::max(g.lds, 64 * 1024 + 1))) return rc;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(g.nqb * g.S)), dim3(ipx::MX_THREADS), g.lds, st, p);
+    IPX_HIP(hipGetLastError());
+    return 0;
+}
+
+void mx4_rows(const ipx_index* ix, ipx::MxParams& p) {
+    p.X = ix->Xx;
+    p.Xs = ix->Xxs;
+    p.N = ix->ntotal;
+    p.d = ix->d;
+    p.nks = ix->nks_x;
+    p.nkq = ix->nkq_x;
+}
+
+// One search pass over the 4-bit rows: pack -> floor (from a sample) -> scan -> the kc best hits -> exact rescoring.
+// The contract of bf16_pass.
+int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* dD, int64_t* dI, hipStream_t st, bool primary,
+             std::vector<int>& flagged, std::vector<int>& hard) {
+    constexpr int PARTS = MX_PARTS_SEARCH, FMT = ipx::MX_E2M3;
+    const int64_t N = ix->ntotal;
+    const int64_t ntiles = (N + ipx::MX_TILE - 1) / ipx::MX_TILE;
+    const bool timing = primary && ix->timing, direct = N <= ipx::MX_DIRECT;
+    const int quad1 = PARTS * ipx::mx_part_bytes<FMT>(32);
+    const MxGeom g = mx4_geometry(ix, nq, quad1, ntiles);
+    // expected hits per query and split: all rows, or the share of the index above the sample's j-th score. j: the
+    // wanted list's share of the sample, m, plus 5 standard deviations of it and a little for short lists — the list
+    // comes out too short (the query is then repeated) with a probability below 1e-7.
+    constexpr int m_rows = ipx::MX_SAMPLE;
+    const double share = (double)kc * m_rows / (double)N;
+    const int j = (int)std::min<double>(m_rows, ceil(share + 5.0 * sqrt(share) + 6.0));
+    const double hits = (double)j * (double)N / m_rows / g.S;
+    // Room per query and split: half as much again and 10 standard deviations; at least one round's rows of a workgroup,
+    // all of which are hits where every score is equal (a zero query: the first rows of the index).
+    const int64_t round_rows = 8 * ipx::MX_TILE;
+    const int64_t cap = direct ? g.rounds * round_rows
+                               : std::min<int64_t>(g.rounds * round_rows, std::max<int64_t>(round_rows, ((int64_t)(1.5 * hits + 10.0 * sqrt(hits)) + 32) / 8 * 8));
+    const size_t info_bytes = ((size_t)nq * sizeof(ipx::MxQueryInfo) + 255) / 256 * 256, word = ((size_t)nq * 4 + 255) / 256 * 256;
+
+    if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
+    if (int rc = ix->cand.ensure((size_t)nq * g.S * cap * sizeof(uint64_t))) return rc;
+    if (int rc = ix->deepN.ensure((size_t)nq * g.S * sizeof(int))) return rc;
+    if (int rc = ix->candD.ensure((size_t)nq * kc * sizeof(float))) return rc;
+    if (int rc = ix->candI.ensure((size_t)nq * kc * sizeof(int64_t))) return rc;
+    if (int rc = ix->mxq.ensure(info_bytes + 4 * word)) return rc;         // norms, row bounds, floors, list states
+    if (!direct)
+        if (int rc = ix->mxs.ensure((size_t)nq * m_rows * sizeof(float))) return rc;
+    if (int rc = ensure_hflags(ix, nq, st)) return rc;
+    ipx::MxQueryInfo* info = (ipx::MxQueryInfo*)ix->mxq.p;
+    int64_t* below = (int64_t*)((char*)ix->mxq.p + info_bytes);
+    float* tau = (float*)((char*)ix->mxq.p + info_bytes + 2 * word);
+    int* todo = (int*)((char*)ix->mxq.p + info_bytes + 3 * word);
+
+    if (timing) IPX_HIP(hipEventRecord(ix->ev[0], st));
+    hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)(g.nqb * 32 * g.cg)), dim3(256), 0, st, (const void*)qf,
+                       (int)IPX_F32, (int)nq, ix->d, PARTS, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, info, todo);
+    IPX_HIP(hipGetLastError());
+    ipx::MxParams p = {};
+    mx4_rows(ix, p);
+    p.Q = (const uint8_t*)ix->Qp.p;
+    p.nq = (int)nq;
+    p.q_dtype = IPX_F32;
+    p.info = info;
+    if (direct) {
+        hipLaunchKernelGGL(ipx::mx4_no_floor_kernel, dim3((unsigned)((nq + 255) / 256)), dim3(256), 0, st, (int)nq, tau, below);
+        IPX_HIP(hipGetLastError());
+    } else {
+        ipx::MxParams ps = p;
+        ps.ntiles = m_rows / ipx::MX_TILE;
+        ps.gstep = (N / ipx::MX_GROUP - 2) / (ps.ntiles - 1);      // whole groups, spread over the index
+        ps.out = (float*)ix->mxs.p;
+        ps.ld = m_rows;
+        ps.row0 = -1;
+        ps.n = m_rows;
+        MxGeom gs = g;
+        gs.S = (int)std::min<int64_t>(g.S, ps.ntiles / 8);
+        if (int rc = launch_mx4_product<PARTS, FMT, ipx::MX_SCORES>(gs, ps, st)) return rc;
+        hipLaunchKernelGGL(ipx::mx4_floor_kernel, dim3((unsigned)nq), dim3(1024), 0, st, (const float*)ix->mxs.p, m_rows, j, N, tau, below);
+        IPX_HIP(hipGetLastError());
+    }
+    if (timing) IPX_HIP(hipEventRecord(ix->ev[1], st));
+    p.gstep = ipx::MX_RG;
+    p.ntiles = ntiles;
+    p.tau = tau;
+    p.row_below = below;
+    p.cand = (uint64_t*)ix->cand.p;
+    p.cnt = (int*)ix->deepN.p;
+    p.todo = todo;
+    p.cap = (int)cap;
+    if (int rc = launch_mx4_product<PARTS, FMT, ipx::MX_SEARCH>(g, p, st)) return rc;
+    if (timing) IPX_HIP(hipEventRecord(ix->ev[2], st));
+    if (int rc = launch_lists_finish(ix, (const uint64_t*)ix->cand.p, (const int*)ix->deepN.p, g.S, (int)cap, kc, nq,
+                                     (float*)ix->candD.p, (int64_t*)ix->candI.p, st))
+        return rc;
+    if (timing) {
+        IPX_HIP(hipEventRecord(ix->ev[3], st));
+        ix->ev_merge = true;
+    }
+    ipx::RescoreParams rp;
+    rp.candD = (const float*)ix->candD.p;
+    rp.candI = (const int64_t*)ix->candI.p;
+    rp.todo = todo;
+    rp.q = qf;
+    rp.qmap = nullptr;
+    rescore_rows(ix, rp);
+    rp.floor = tau;
+    rp.maxsq = (const uint32_t*)ix->maxsq.p;
+    rp.outD = dD;
+    rp.outI = dI;
+    rp.flags = ix->hflags;
+    rp.err = (const int*)ix->err.p;
+    rp.outl_count = nullptr;
+    rp.shared_list = 0;
+    rp.nq = (int)nq;
+    rp.id_base = ix->id_base;
+    rp.acc_coef = margin_acc_coef(ix->nks_x * ipx::MX_KSET, PARTS);
+    rp.qparts = PARTS;
+    rp.post = ix->margin_post;
+    rp.d = ix->d;
+    rp.k = k;
+    rp.kc = kc;
+    rp.P = next_pow2(kc);
+    if (int rc = launch_rescore(rp, nq, st)) return rc;
+    if (timing) {
+        IPX_HIP(hipEventRecord(ix->ev[4], st));
+        ix->ev_rescore = true;
+    }
+    if (primary) {
+        ix->ev_valid = ix->timing;
+        ix->last_wgs = g.nqb * g.S;
+        ix->last_S = g.S;
+        ix->last_cap = (int)cap;
+        ix->last_kc = kc;
+    }
+    IPX_HIP(hipStreamSynchronize(st));
+    flagged.clear();
+    hard.clear();
+    for (int64_t i = 0; i < nq; ++i)
+        if (ix->hflags[i]) (ix->hflags[i] == 2 ? hard : flagged).push_back((int)i);
+    return 0;
+}
+
+// Search of an mx4 index: what a bf16 index of the same values returns, bit for bit. Queries whose list cannot be proven
+// sufficient are repeated with the longest one, and what still fails is answered from every stored row.
+int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int logits, int64_t nq, int k, float* dD, int64_t* dI,
+                  hipStream_t st) {
+    const float* qf = dq;
+    if (A > 0)
+        if (int rc = fuse_queries(ix, dq, dw, A, logits, nq, st, &qf)) return rc;
+    const int kc0 = ix->force_kc > 0 ? ix->force_kc : std::max(128, k + k / 2);
+    const int kc = std::min(std::max(kc0, k), MAX_KC);
+    for (int64_t q0 = 0; q0 < nq; q0 += MX_SLICE) {
+        const int64_t n = std::min<int64_t>(MX_SLICE, nq - q0);
+        const float* q = qf + q0 * ix->d;
+        float* D = dD + q0 * k;
+        int64_t* I = dI + q0 * k;
+        std::vector<int> flagged, hard;
+        if (int rc = mx4_pass(ix, q, n, k, kc, D, I, st, q0 == 0, flagged, hard)) return rc;
+        ix->last_fallback += (int64_t)(flagged.size() + hard.size());
+        if (!flagged.empty()) {
+            std::vector<int> still, still_hard;
+            int rc = redo_queries(ix, q, flagged, k, D, I, st, [&](const float* q2, int64_t n2, float* D2, int64_t* I2) {
+                return mx4_pass(ix, q2, n2, k, MAX_KC, D2, I2, st, false, still, still_hard);
+            });
+            if (rc) return rc;
+            still.insert(still.end(), still_hard.begin(), still_hard.end());
+            for (int& i : still) i = flagged[(size_t)i];
+            hard.insert(hard.end(), still.begin(), still.end());
+        }
+        if (hard.empty()) continue;
+        ix->last_exact += (int64_t)hard.size();
+        std::sort(hard.begin(), hard.end());
+        // (the repeat pass has put other queries' norms where the rescoring kernel reads them)
+        if (int rc = ix->Qp.ensure((size_t)((n + 31) / 32) * ix->nkq_x * ipx::mx_part_bytes<ipx::MX_E2M3>(32))) return rc;
+        if (int rc = ix->mxq.ensure((size_t)n * sizeof(ipx::MxQueryInfo))) return rc;
+        hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)n), dim3(256), 0, st, (const void*)q, (int)IPX_F32, (int)n,
+                           ix->d, 1, 32, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr);
+        IPX_HIP(hipGetLastError());
+        if (int rc = exact_rows_path(ix, q, hard, k, D, I, st)) return rc;
+    }
+    return 0;
+}
+
+// S = Q X^T over rows [row0, row0 + n) of an mx4 index; out: device, [nq][n].
+int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_scales, int64_t nq, int64_t row0, int64_t n, float* out,
+                hipStream_t st) {
+    ipx::MxParams p = {};
+    mx4_rows(ix, p);
+    p.g0 = row0 / ipx::MX_TILE * ipx::MX_RG;             // whole tiles: the buffers end behind one
+    p.gstep = ipx::MX_RG;
+    p.ntiles = (row0 + n + ipx::MX_TILE - 1) / ipx::MX_TILE - row0 / ipx::MX_TILE;
+    p.nq = (int)nq;
+    p.out = out;
+    p.ld = n;
+    p.row0 = row0;
+    p.n = n;
+    if (q_scales) {
+        const int quad1 = ipx::mx_part_bytes<ipx::MX_E2M1>(32);
+        const MxGeom g = mx4_geometry(ix, nq, quad1, p.ntiles);
+        if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
+        const int64_t total = (int64_t)g.nqb * 32 * g.cg * ix->nkq_x * 8;
+        hipLaunchKernelGGL(ipx::mx4_pack_codes_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, (const uint8_t*)dq,
+                           q_scales, (int)nq, ix->d, 32 * g.cg, ix->nkq_x, total, (uint8_t*)ix->Qp.p);
+        IPX_HIP(hipGetLastError());
+        p.Q = (const uint8_t*)ix->Qp.p;
+        return launch_mx4_product<1, ipx::MX_E2M1, ipx::MX_SCORES>(g, p, st);
+    }
+    const int quad1 = MX_PARTS_SCORES * ipx::mx_part_bytes<ipx::MX_E2M3>(32);
+    const MxGeom g = mx4_geometry(ix, nq, quad1, p.ntiles);
+    if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
+    if (int rc = ix->mxq.ensure((size_t)nq * sizeof(ipx::MxQueryInfo))) return rc;
+    hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)(g.nqb * 32 * g.cg)), dim3(256), 0, st, dq, q_dtype, (int)nq,
+                       ix->d, MX_PARTS_SCORES, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr);
+    IPX_HIP(hipGetLastError());
+    p.Q = (const uint8_t*)ix->Qp.p;
+    p.q = dq;
+    p.q_dtype = q_dtype;
+    p.info = (const ipx::MxQueryInfo*)ix->mxq.p;
+    return launch_mx4_product<MX_PARTS_SCORES, ipx::MX_E2M3, ipx::MX_SCORES>(g, p, st);
 }
 
 // Shared body of ipx_search / ipx_search_aspect. q_src is [nq, d] (A == 0) or [nq, A, d].
@@ -1281,6 +1660,8 @@ int search_impl(ipx_index* ix, const float* q_src, const float* w, int A, int lo
         // storage does not have. A forced candidate count ("bf16_candidates") changes the list length, never these
         // limits.
         const int bf16_max_k = ipx::DEEP_MAX_K / 2;
+        if (ix->storage == 3 && k > MX_MAX_K)
+            return fail(IPX_ERR_ARG, "search: mx4 storage serves k <= " + std::to_string(MX_MAX_K) + "; use storage 0 or 1 for deeper searches");
         const bool deep_rows_fit = (ix->storage == 2 ? ix->nks_h * 32 : ix->nks * 16) <= 2048;
         const int bf16_limit = deep_rows_fit ? bf16_max_k : IPX_MAX_K * 4 / 5;
         if (ix->storage == 2 && k > bf16_limit)
@@ -1291,7 +1672,8 @@ int search_impl(ipx_index* ix, const float* q_src, const float* w, int A, int lo
         const bool bf16 = ix->storage == 2 ||
                           (ix->storage == 1 && !ix->force_f32_scan && k <= (deep_rows_fit ? bf16_max_k : IPX_MAX_K) &&
                            k < ix->bf16_fail_k);
-        int rc = bf16 ? scan_bf16_path(ix, dq, dw, A, logits, nq, k, dD, dI, st)
+        int rc = ix->storage == 3 ? scan_mx4_path(ix, dq, dw, A, logits, nq, k, dD, dI, st)
+                 : bf16 ? scan_bf16_path(ix, dq, dw, A, logits, nq, k, dD, dI, st)
                  : k > ipx::DEEP_MAX_K ? scan_f32_deep(ix, dq, dw, A, logits, nq, k, dD, dI, st)
                                  : scan_f32_path(ix, dq, dw, A, logits, nq, k, dD, dI, st, true);
         if (rc) return rc;
@@ -1406,6 +1788,8 @@ int ipx_create(int d, int device, ipx_index** out) {
     ix->d = d;
     ix->nks = (d + ipx::BK - 1) / ipx::BK;
     ix->nks_h = (d + ipx::HBK - 1) / ipx::HBK;
+    ix->nks_x = (d + ipx::MX_KSET - 1) / ipx::MX_KSET;
+    ix->nkq_x = (ix->nks_x + 3) / 4;
     ix->device = device;
     int cus = 0;
     hipError_t e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
@@ -1446,9 +1830,11 @@ int ipx_destroy(ipx_index* ix) {
     DeviceGuard guard(ix->device);
     if (ix->Xp) (void)hipFree(ix->Xp);
     if (ix->Xh) (void)hipFree(ix->Xh);
+    if (ix->Xx) (void)hipFree(ix->Xx);
+    if (ix->Xxs) (void)hipFree(ix->Xxs);
     for (DevBuf* b : {&ix->Qp, &ix->cand, &ix->partD, &ix->partI, &ix->err, &ix->stageIn, &ix->stageQ, &ix->stageW,
                       &ix->outD, &ix->outI, &ix->trace, &ix->pub, &ix->maxsq, &ix->outl, &ix->olist, &ix->sideD, &ix->sideI, &ix->qfused, &ix->candD, &ix->candI, &ix->deepD, &ix->deepI, &ix->ceilD, &ix->ceilI, &ix->deepK, &ix->deepN,
-                      &ix->flags, &ix->sel, &ix->qsel, &ix->selD, &ix->selI, &ix->poolH, &ix->poolW, &ix->poolQ})
+                      &ix->flags, &ix->sel, &ix->qsel, &ix->selD, &ix->selI, &ix->poolH, &ix->poolW, &ix->poolQ, &ix->mxq, &ix->mxs})
         b->release();
     for (auto& e : ix->ev)
         if (e) (void)hipEventDestroy(e);
@@ -1544,6 +1930,207 @@ int ipx_add(ipx_index* ix, const void* rows, int64_t n, int dtype, int on_device
     return 0;
 }
 
+int ipx_add_mx4(ipx_index* ix, const uint8_t* codes, const uint8_t* scales, int64_t n, int on_device, void* stream) {
+    if (!ix) return fail(IPX_ERR_ARG, "add_mx4: null index");
+    if (n < 0) return fail(IPX_ERR_ARG, "add_mx4: n < 0");
+    if (ix->storage != 3) return fail(IPX_ERR_STATE, "add_mx4: needs mx4 storage (ipx_set_param \"storage\" 3)");
+    if (n == 0) return 0;
+    if (!codes || !scales) return fail(IPX_ERR_ARG, "add_mx4: null pointer");
+    if (ix->ntotal + n > (int64_t)0x7fffff00) return fail(IPX_ERR_ARG, "add_mx4: more than 2^31 rows in one index");
+    IPX_ON_DEVICE(ix->device);
+    hipStream_t st = (hipStream_t)stream;
+    if (int rc = grow_storage(ix, ix->ntotal + n, st)) return rc;
+    const int nb = (ix->d + 31) / 32;
+    // host rows travel in slices of 256 MiB
+    const int64_t slice = on_device ? rows_per_launch(nb) : std::max<int64_t>(1, (256ll << 20) / (17 * nb));
+    for (int64_t r0 = 0; r0 < n; r0 += slice) {
+        const int64_t m = std::min(slice, n - r0);
+        const uint8_t *c = codes + (size_t)r0 * nb * 16, *s = scales + (size_t)r0 * nb;
+        if (!on_device) {
+            const size_t cb = (size_t)m * nb * 16, sb = (size_t)m * nb;
+            if (int rc = ix->stageIn.ensure(cb + sb)) return rc;
+            IPX_HIP(hipMemcpyAsync(ix->stageIn.p, c, cb, hipMemcpyHostToDevice, st));
+            IPX_HIP(hipMemcpyAsync((char*)ix->stageIn.p + cb, s, sb, hipMemcpyHostToDevice, st));
+            c = (const uint8_t*)ix->stageIn.p;
+            s = c + cb;
+        }
+        const uint32_t total = (uint32_t)(m * nb);
+        hipLaunchKernelGGL(ipx::mx4_place_kernel, dim3((total + 255) / 256), dim3(256), 0, st, c, s, total, magic_of(nb), nb, ix->d,
+                           ix->Xx, ix->Xxs, ix->ntotal + r0, ix->nks_x, ix->nkq_x);
+        IPX_HIP(hipGetLastError());
+    }
+    if (int rc = launch_mx4_norms(ix, ix->ntotal, n, st)) return rc;
+    if (!on_device) IPX_HIP(hipStreamSynchronize(st));
+    ix->ntotal += n;
+    return 0;
+}
+
+// ipx_scores / ipx_scores_mx4 (q_scales != null: mx4 queries)
+static int scores_impl(ipx_index* ix, const char* who, const void* q, int q_dtype, const uint8_t* q_scales, bool mx4, int64_t nq,
+                       int64_t row0, int64_t n, float* out, int on_device, void* stream) {
+    const std::string w(who);
+    if (!ix) return fail(IPX_ERR_ARG, w + ": null index");
+    if (!mx4 && q_dtype != IPX_F32 && q_dtype != IPX_F16 && q_dtype != IPX_BF16) return fail(IPX_ERR_ARG, w + ": unknown dtype");
+    if (ix->storage != 3) return fail(IPX_ERR_STATE, w + ": needs mx4 storage (ipx_set_param \"storage\" 3)");
+    if (nq < 0 || nq > 0x7fffff00) return fail(IPX_ERR_ARG, w + ": nq outside [0, 2^31 - 256]");
+    if (row0 < 0 || n < 0 || row0 > ix->ntotal || n > ix->ntotal - row0)
+        return fail(IPX_ERR_ARG, w + ": rows [" + std::to_string(row0) + ", " + std::to_string(row0) + " + " + std::to_string(n) +
+                    ") outside the index of " + std::to_string(ix->ntotal));
+    if (nq == 0 || n == 0) return 0;
+    if (!q || !out || (mx4 && !q_scales)) return fail(IPX_ERR_ARG, w + ": null pointer");
+    IPX_ON_DEVICE(ix->device);
+    hipStream_t st = (hipStream_t)stream;
+    if (on_device) return scores_path(ix, q, q_dtype, q_scales, nq, row0, n, out, st);
+    const size_t nb = (size_t)(ix->d + 31) / 32;
+    const size_t qb = mx4 ? (size_t)nq * nb * 16 : (size_t)nq * ix->d * dtype_size(q_dtype), sb = mx4 ? (size_t)nq * nb : 0;
+    const size_t ob = (size_t)nq * n * sizeof(float);
+    if (int rc = ix->stageQ.ensure(qb + sb)) return rc;
+    if (int rc = ix->outD.ensure(ob)) return rc;
+    IPX_HIP(hipMemcpyAsync(ix->stageQ.p, q, qb, hipMemcpyHostToDevice, st));
+    if (mx4) IPX_HIP(hipMemcpyAsync((char*)ix->stageQ.p + qb, q_scales, sb, hipMemcpyHostToDevice, st));
+    if (int rc = scores_path(ix, ix->stageQ.p, q_dtype, mx4 ? (const uint8_t*)ix->stageQ.p + qb : nullptr, nq, row0, n, (float*)ix->outD.p, st))
+        return rc;
+    IPX_HIP(hipMemcpyAsync(out, ix->outD.p, ob, hipMemcpyDeviceToHost, st));
+    IPX_HIP(hipStreamSynchronize(st));
+    return 0;
+}
+
+int ipx_scores(ipx_index* ix, const void* q, int q_dtype, int64_t nq, int64_t row0, int64_t n, float* out, int on_device, void* stream) {
+    return scores_impl(ix, "scores", q, q_dtype, nullptr, false, nq, row0, n, out, on_device, stream);
+}
+
+int ipx_scores_mx4(ipx_index* ix, const uint8_t* q_codes, const uint8_t* q_scales, int64_t nq, int64_t row0, int64_t n, float* out,
+                   int on_device, void* stream) {
+    return scores_impl(ix, "scores_mx4", q_codes, IPX_F32, q_scales, true, nq, row0, n, out, on_device, stream);
+}
+
+int ipx_lookup(ipx_index* ix, const int64_t* ids, int64_t n, const float* scale, void* out, int dtype, int on_device, void* stream) {
+    if (!ix) return fail(IPX_ERR_ARG, "lookup: null index");
+    if (n < 0) return fail(IPX_ERR_ARG, "lookup: n < 0");
+    if (dtype != IPX_F32 && dtype != IPX_F16 && dtype != IPX_BF16) return fail(IPX_ERR_ARG, "lookup: unknown dtype");
+    if (n == 0) return 0;
+    if (!ids || !out) return fail(IPX_ERR_ARG, "lookup: null pointer");
+    const int d = ix->d, np = (d + 7) / 8;
+    const size_t row_bytes = (size_t)d * dtype_size(dtype);
+    if (!on_device)
+        for (int64_t i = 0; i < n; ++i) {
+            const uint64_t row = (uint64_t)ids[i] - (uint64_t)ix->id_base;
+            if (ids[i] != -1 && row >= (uint64_t)ix->ntotal)
+                return fail(IPX_ERR_ARG, "lookup: id " + std::to_string(ids[i]) + " is neither -1 nor a row of the index");
+        }
+    IPX_ON_DEVICE(ix->device);
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t* di = ids;
+    const float* ds = scale;
+    char* dout = (char*)out;
+    if (!on_device) {
+        const size_t ib = (size_t)n * sizeof(int64_t), sb = scale ? (size_t)n * sizeof(float) : 0;
+        if (int rc = ix->stageQ.ensure(ib + sb)) return rc;
+        if (int rc = ix->outD.ensure((size_t)n * row_bytes)) return rc;
+        IPX_HIP(hipMemcpyAsync(ix->stageQ.p, ids, ib, hipMemcpyHostToDevice, st));
+        if (scale) IPX_HIP(hipMemcpyAsync((char*)ix->stageQ.p + ib, scale, sb, hipMemcpyHostToDevice, st));
+        di = (const int64_t*)ix->stageQ.p;
+        ds = scale ? (const float*)((char*)ix->stageQ.p + ib) : nullptr;
+        dout = (char*)ix->outD.p;
+    } else {
+        ix->lookups = true;
+    }
+    const int xfmt = ix->storage == 3 ? 2 : ix->storage == 2 ? 1 : 0;
+    const void* X = xfmt == 2 ? (const void*)ix->Xx : xfmt ? (const void*)ix->Xh : (const void*)ix->Xp;
+    const int nks = xfmt == 2 ? ix->nks_x : xfmt ? ix->nks_h : ix->nks;
+    const bool wide = aligned16(dout) && row_bytes % 16 == 0;
+    const int64_t slice = rows_per_launch(np);
+    for (int64_t i0 = 0; i0 < n; i0 += slice) {
+        const uint32_t total = (uint32_t)(std::min(slice, n - i0) * np);
+        hipLaunchKernelGGL(ipx::lookup_kernel, dim3((total + 255) / 256), dim3(256), 0, st, X, (const uint8_t*)ix->Xxs, xfmt, nks,
+                           ix->nkq_x, ix->id_base, ix->ntotal, di + i0, ds ? ds + i0 : nullptr, total, magic_of(np), np, d,
+                           (void*)(dout + (size_t)i0 * row_bytes), dtype, wide, (int*)ix->err.p + LOOKUP_ERR);
+        IPX_HIP(hipGetLastError());
+    }
+    if (!on_device) {
+        IPX_HIP(hipMemcpyAsync(out, dout, (size_t)n * row_bytes, hipMemcpyDeviceToHost, st));
+        IPX_HIP(hipStreamSynchronize(st));
+    }
+    return 0;
+}
+
+int ipx_mx4_quantize(const void* rows, int64_t n, int d, int64_t stride, int dtype, uint8_t* codes, uint8_t* scales, int on_device,
+                     int device, void* stream) {
+    if (n < 0) return fail(IPX_ERR_ARG, "mx4_quantize: n < 0");
+    if (d <= 0 || d > 65536) return fail(IPX_ERR_ARG, "mx4_quantize: dimension " + std::to_string(d) + " outside [1, 65536]");
+    if (dtype != IPX_F32 && dtype != IPX_F16 && dtype != IPX_BF16) return fail(IPX_ERR_ARG, "mx4_quantize: unknown dtype");
+    if (stride < d && n > 1) return fail(IPX_ERR_ARG, "mx4_quantize: stride shorter than a row");
+    if (n == 0) return 0;
+    if (!rows || !codes || !scales) return fail(IPX_ERR_ARG, "mx4_quantize: null pointer");
+    if (((uintptr_t)codes & 3) != 0) return fail(IPX_ERR_ARG, "mx4_quantize: codes must start at a multiple of 4 bytes");
+    IPX_ON_DEVICE(device);
+    hipStream_t st = (hipStream_t)stream;
+    if (on_device) return launch_mx4_quantize(rows, dtype, n, d, stride, codes, scales, nullptr, 0, st);
+    const size_t nb = (size_t)(d + 31) / 32, el = dtype_size(dtype), rb = ((size_t)(n - 1) * stride + d) * el, cb = (size_t)n * nb * 16, sb = (size_t)n * nb;
+    DevBuf in, o;
+    int rc = in.ensure(rb);
+    if (!rc) rc = o.ensure(cb + sb);
+    hipError_t e = hipSuccess;
+    if (!rc) {
+        e = hipMemcpyAsync(in.p, rows, rb, hipMemcpyHostToDevice, st);
+        if (e == hipSuccess) rc = launch_mx4_quantize(in.p, dtype, n, d, stride, (uint8_t*)o.p, (uint8_t*)o.p + cb, nullptr, 0, st);
+        if (e == hipSuccess && !rc) e = hipMemcpyAsync(codes, o.p, cb, hipMemcpyDeviceToHost, st);
+        if (e == hipSuccess && !rc) e = hipMemcpyAsync(scales, (char*)o.p + cb, sb, hipMemcpyDeviceToHost, st);
+        const hipError_t e2 = hipStreamSynchronize(st);
+        if (e == hipSuccess) e = e2;
+    }
+    in.release();
+    o.release();
+    if (rc) return rc;
+    if (e != hipSuccess) return fail(IPX_ERR_HIP, std::string("mx4_quantize: ") + hipGetErrorString(e));
+    return 0;
+}
+
+int ipx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n, int d, void* out, int dtype, int on_device, int device,
+                       void* stream) {
+    if (n < 0) return fail(IPX_ERR_ARG, "mx4_dequantize: n < 0");
+    if (d <= 0 || d > 65536) return fail(IPX_ERR_ARG, "mx4_dequantize: dimension " + std::to_string(d) + " outside [1, 65536]");
+    if (dtype != IPX_F32 && dtype != IPX_F16 && dtype != IPX_BF16) return fail(IPX_ERR_ARG, "mx4_dequantize: unknown dtype");
+    if (n == 0) return 0;
+    if (!codes || !scales || !out) return fail(IPX_ERR_ARG, "mx4_dequantize: null pointer");
+    IPX_ON_DEVICE(device);
+    hipStream_t st = (hipStream_t)stream;
+    const size_t nb = (size_t)(d + 31) / 32, cb = (size_t)n * nb * 16, sb = (size_t)n * nb, row_bytes = (size_t)d * dtype_size(dtype);
+    DevBuf in, o;
+    const uint8_t *dc = codes, *ds = scales;
+    char* dout = (char*)out;
+    hipError_t e = hipSuccess;
+    if (!on_device) {
+        int rc = in.ensure(cb + sb);
+        if (!rc) rc = o.ensure((size_t)n * row_bytes);
+        if (rc) { in.release(); o.release(); return rc; }
+        e = hipMemcpyAsync(in.p, codes, cb, hipMemcpyHostToDevice, st);
+        if (e == hipSuccess) e = hipMemcpyAsync((char*)in.p + cb, scales, sb, hipMemcpyHostToDevice, st);
+        dc = (const uint8_t*)in.p;
+        ds = dc + cb;
+        dout = (char*)o.p;
+    }
+    const int np = (d + 7) / 8;
+    // (the wide form also reads the codes as dwords: they then start at a multiple of 4 bytes)
+    const bool wide = aligned16(dout) && row_bytes % 16 == 0 && ((uintptr_t)dc & 3) == 0;
+    const int64_t slice = rows_per_launch(np);
+    for (int64_t r0 = 0; r0 < n && e == hipSuccess; r0 += slice) {
+        const uint32_t total = (uint32_t)(std::min(slice, n - r0) * np);
+        hipLaunchKernelGGL(ipx::mx4_dequantize_kernel, dim3((total + 255) / 256), dim3(256), 0, st, dc + (size_t)r0 * nb * 16,
+                           ds + (size_t)r0 * nb, total, magic_of(np), np, d, (int)nb, (void*)(dout + (size_t)r0 * row_bytes), dtype, wide);
+        e = hipGetLastError();
+    }
+    if (!on_device) {
+        if (e == hipSuccess) e = hipMemcpyAsync(out, dout, (size_t)n * row_bytes, hipMemcpyDeviceToHost, st);
+        const hipError_t e2 = hipStreamSynchronize(st);
+        if (e == hipSuccess) e = e2;
+        in.release();
+        o.release();
+    }
+    if (e != hipSuccess) return fail(IPX_ERR_HIP, std::string("mx4_dequantize: ") + hipGetErrorString(e));
+    return 0;
+}
+
 int ipx_search(ipx_index* ix, const float* q, int64_t nq, int k, float* out_D, int64_t* out_I, int on_device,
                void* stream) {
     return search_impl(ix, q, nullptr, 0, 0, nq, k, out_D, out_I, on_device, stream);
@@ -1559,7 +2146,7 @@ int ipx_search_noalloc(ipx_index* ix, const float* q, int64_t nq, int k, float* 
                     std::to_string(IPX_NOALLOC_MAX_QUERIES) + "] (use ipx_search for larger batches)");
     if (k <= 0 || k > IPX_MAX_K)
         return fail(IPX_ERR_ARG, "search_noalloc: k=" + std::to_string(k) + " outside [1, " + std::to_string(IPX_MAX_K) + "]");
-    if (ix->storage == 2) return fail(IPX_ERR_STATE, "search_noalloc: needs fp32 rows (storage 0 or 1)");
+    if (ix->storage >= 2) return fail(IPX_ERR_STATE, "search_noalloc: needs fp32 rows (storage 0 or 1)");
     if (nq == 0) return 0;
     if (!q || !out_D || !out_I) return fail(IPX_ERR_ARG, "search_noalloc: null pointer");
     DeviceGuard guard(ix->device);
@@ -1793,10 +2380,10 @@ int ipx_set_param(ipx_index* ix, const char* name, int64_t value) {
         return 0;
     }
     if (!strcmp(name, "storage")) {
-        if (value < 0 || value > 2) return fail(IPX_ERR_ARG, "set_param: storage must be 0 (f32), 1 (f32 + bf16 scan) or 2 (bf16)");
-        if (ix->ntotal > 0 || ix->cap_tiles > 0 || ix->cap_tiles_h > 0)
+        if (value < 0 || value > 3) return fail(IPX_ERR_ARG, "set_param: storage must be 0 (f32), 1 (f32 + bf16 scan), 2 (bf16) or 3 (mx4)");
+        if (ix->ntotal > 0 || ix->cap_tiles > 0 || ix->cap_tiles_h > 0 || ix->cap_groups_x > 0)
             return fail(IPX_ERR_STATE, "set_param: storage can only be chosen while the index is empty and unreserved");
-        if (value != 0 && ix->d > 8192) return fail(IPX_ERR_ARG, "set_param: bf16 storage needs d <= 8192");
+        if (value != 0 && ix->d > 8192) return fail(IPX_ERR_ARG, "set_param: bf16 and mx4 storage need d <= 8192");
         ix->storage = (int)value;
         return 0;
     }
@@ -1875,7 +2462,7 @@ int ipx_set_param(ipx_index* ix, const char* name, int64_t value) {
         return 0;
     }
     if (!strcmp(name, "f32_scan")) {
-        if (value && ix->storage == 2) return fail(IPX_ERR_STATE, "set_param: f32_scan needs fp32 rows (storage 0 or 1)");
+        if (value && ix->storage >= 2) return fail(IPX_ERR_STATE, "set_param: f32_scan needs fp32 rows (storage 0 or 1)");
         ix->force_f32_scan = value != 0;
         return 0;
     }
@@ -1915,6 +2502,14 @@ int ipx_check(ipx_index* ix, void* stream) {
     if (errflag) {
         (void)hipMemsetAsync(ix->last_err, 0, sizeof(int), st);
         return fail(IPX_ERR_STATE, "search: candidate queue overflow (internal invariant violated)");
+    }
+    if (ix->lookups) {
+        int bad = 0;
+        IPX_HIP(hipMemcpy(&bad, (int*)ix->err.p + LOOKUP_ERR, sizeof(int), hipMemcpyDeviceToHost));
+        if (bad) {
+            (void)hipMemset((int*)ix->err.p + LOOKUP_ERR, 0, sizeof(int));
+            return fail(IPX_ERR_ARG, "lookup: an id was neither -1 nor a row of the index (its row was filled with zeros)");
+        }
     }
     return 0;
 }

@@ -898,7 +898,7 @@ struct RescoreParams {
     const float* q;          // [nq][d] fp32 queries, row-major
     const int* qmap;         // optional: list qi belongs to query qmap[qi] (exact_rows_path: many lists, one query)
     int shared_list;         // 1: every query rescoring the same list candD / candI [kc] (the outlier rows)
-    const void* X;           // packed corpus: fp32 (tiles of 128) or bf16 (tiles of 256)
+    const void* X;           // packed corpus: fp32 (tiles of 128), bf16 (tiles of 256) or mx4 codes (groups of 32)
     const uint32_t* maxsq;   // float bits of max_x |x|^2 and max_x |x - bf16(x)|^2
     float* outD;             // [nq][k]
     int64_t* outI;           // [nq][k]
@@ -911,7 +911,12 @@ struct RescoreParams {
     float acc_coef;          // accumulation-error coefficient (host: margin_acc_coef)
     int qparts;              // bf16 parts of the query the scan used (1: hi, 2: hi + lo)
     int post;                // 1: try the after-the-fact margin test when the a-priori one fails
-    int d, nks, x_is_bf16, k, kc, P;
+    int d, nks, xfmt, k, kc, P;           // xfmt: 0 fp32 rows, 1 bf16 rows, 2 mx4 rows
+    // mx4 rows only
+    const uint8_t* Xs = nullptr;          // their scales
+    int nkq = 0;
+    const float* qinfo = nullptr;         // [nq][2]: |q|^2 and |q - scanned parts|^2 (mx4_pack_queries_kernel)
+    const float* floor = nullptr;         // [nq]: the score a candidate had to reach; -FLT_MAX: none
 };
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
@@ -924,12 +929,12 @@ constexpr int RS_RANK_SORT = 1024;   // lists of up to this many scored candidat
 // NW waves per query: 4 for large batches (the chip is full of workgroups anyway), 16 for small ones, where a query's
 // workgroup is alone on its CU and the time is the latency of its dependent rounds — 256 candidates in flight per
 // round instead of 64. The rows' K-stages are fetched one group ahead of the fmaf chains that consume them.
-template <int NW>
+template <int NW, bool MX4 = false>
 __global__ void __launch_bounds__(NW * 64)
 rescore_kernel(const RescoreParams p) {
     constexpr int NT = NW * 64;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int dpad = p.nks * (p.x_is_bf16 ? 32 : 16);
+    const int dpad = MX4 ? (p.nks + 1) / 2 * 128 : p.nks * (p.xfmt ? 32 : 16);
     float* qs = (float*)smem;                                  // [dpad]
     uint64_t* keys = (uint64_t*)(smem + (size_t)((dpad * 4 + 15) & ~15));   // [P]
     __shared__ float red[2 * NW];
@@ -953,6 +958,11 @@ rescore_kernel(const RescoreParams p) {
     __syncthreads();
     float qn2 = 0.f, dqn2 = 0.f;
     for (int w = 0; w < NW; ++w) { qn2 += red[w]; dqn2 += red[NW + w]; }
+    if constexpr (MX4) {
+        const int64_t qq = p.qmap ? (int64_t)p.qmap[qi] : qi;
+        qn2 = p.qinfo[2 * qq];
+        dqn2 = p.qinfo[2 * qq + 1];
+    }
     const float qn = sqrtf(qn2);
     const float dqn = sqrtf(dqn2);
     const float Mx = sqrtf(__uint_as_float(p.maxsq[0])), Dx = sqrtf(__uint_as_float(p.maxsq[1]));
@@ -1002,10 +1012,14 @@ rescore_kernel(const RescoreParams p) {
             // the outlier rows: every listed row is scored, nothing was cut off
         } else if (!tame) {
             flag = 2;
-        } else if (eps == 0.f) {
+        } else if (eps == 0.f && (!MX4 || p.floor)) {
+            // (mx4 rows: not on lists that enumerate the index, which hold rows of NaNs too)
             // a zero query (or an all-zero index): every approximate score IS the exact score, the list is in the
             // result order (score desc, id asc) already — its first k entries are the answer, whatever ties follow
             m = nvalid < p.k ? nvalid : p.k;
+            if (MX4 && m < p.k && p.floor && p.floor[qi] > -FLT_MAX) flag = 1;
+        } else if (MX4 && nvalid < p.kc && p.floor && p.floor[qi] > -FLT_MAX) {
+            flag = 1;                               // fewer rows than asked for reached the floor: others may belong here
         } else if (nvalid >= p.kc) {                // the list is full: it may have cut rows off
             if (s_nge < p.kc && s_nge >= p.k) {     // its last score lies below thr: everything from there on is cut
                 m = s_nge;                          // (the k-th score itself is >= thr; a NaN thr counts nothing: flagged)
@@ -1036,7 +1050,59 @@ rescore_kernel(const RescoreParams p) {
     const bool by_rank = p.P <= RS_RANK_SORT;
     uint64_t* sorted = keys + p.P;                            // [P] when by_rank
     char* stage = (char*)(sorted + (by_rank ? p.P : 0)) + wave * (RS_KB * 16 * RS_ROW);
-    const int R = p.x_is_bf16 ? HBD : BD;                 // rows per tile of the packed layout
+    if constexpr (MX4) {
+        // The same with mx4 rows: a line is 128 elements (two K-sets), four blocks of 16 bytes; lane r < 16 also loads its
+        // row's scales, four dwords a round. A block's values are codes times a power of two: exact, so the chain is the
+        // one a bf16 index of these values runs.
+        const int nb = (p.d + 31) / 32, nlines = (p.nks + 1) / 2;
+        for (int g0 = wave * 16; g0 < m; g0 += NW * 16) {
+            const int r = lane >> 2, pc = lane & 3;
+            const int64_t row = cI[g0 + r < m ? g0 + r : m - 1] - p.id_base;
+            const char* src = (const char*)p.X + (size_t)(row >> 5) * p.nks * 1024 + (row & 31) * 32 + (pc & 1) * 16;
+            const int my = g0 + lane < m ? g0 + lane : m - 1;
+            const int64_t myrow = lane < 16 ? cI[my] - p.id_base : 0;
+            const uint32_t* sp = (const uint32_t*)(p.Xs + (size_t)myrow * p.nkq * 8);
+            float acc = 0.f;
+            const int last = p.nks - 1;
+            auto fetch = [&](int line) { const int ks = 2 * line + (pc >> 1); return *(const uint4*)(src + (size_t)(ks < last ? ks : last) * 1024); };
+            auto scales = [&](int i) { return lane < 16 ? sp[i < 2 * p.nkq ? i : 2 * p.nkq - 1] : 0u; };
+            uint4 v0 = fetch(0), v1 = fetch(1), v2 = fetch(2), v3 = fetch(3);
+            uint32_t s0 = scales(0), s1 = scales(1), s2 = scales(2), s3 = scales(3);
+            for (int l0 = 0; l0 < nlines; l0 += 4) {
+                *(uint4*)(stage + (0 * 16 + r) * RS_ROW + pc * 16) = v0;
+                *(uint4*)(stage + (1 * 16 + r) * RS_ROW + pc * 16) = v1;
+                *(uint4*)(stage + (2 * 16 + r) * RS_ROW + pc * 16) = v2;
+                *(uint4*)(stage + (3 * 16 + r) * RS_ROW + pc * 16) = v3;
+                const uint32_t c0 = s0, c1 = s1, c2 = s2, c3 = s3;
+                v0 = fetch(l0 + 4); v1 = fetch(l0 + 5); v2 = fetch(l0 + 6); v3 = fetch(l0 + 7);
+                s0 = scales(l0 + 4); s1 = scales(l0 + 5); s2 = scales(l0 + 6); s3 = scales(l0 + 7);
+                wave_lds_sync();
+                if (lane < 16) {
+                    const int blocks = nb - l0 * 4 < 16 ? nb - l0 * 4 : 16;
+                    for (int b = 0; b < blocks; ++b) {             // block b: K-set b >> 1, half b & 1
+                        const uint32_t word = b & 8 ? (b & 1 ? c3 : c2) : (b & 1 ? c1 : c0);
+                        const uint32_t byte = (word >> (8 * ((b >> 1) & 3))) & 255u;
+                        const float sc = __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
+                        const uint4 w = *(const uint4*)(stage + ((b >> 2) * 16 + lane) * RS_ROW + (b & 3) * 16);
+                        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float* qq = qs + (l0 * 4 + b) * 32 + i * 8;
+                            const auto e01 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], 1.f, 0), e23 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], 1.f, 1);
+                            const auto e45 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], 1.f, 2), e67 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], 1.f, 3);
+                            acc = fmaf(e01[0] * sc, qq[0], acc); acc = fmaf(e45[0] * sc, qq[4], acc);
+                            acc = fmaf(e01[1] * sc, qq[1], acc); acc = fmaf(e45[1] * sc, qq[5], acc);
+                            acc = fmaf(e23[0] * sc, qq[2], acc); acc = fmaf(e67[0] * sc, qq[6], acc);
+                            acc = fmaf(e23[1] * sc, qq[3], acc); acc = fmaf(e67[1] * sc, qq[7], acc);
+                        }
+                    }
+                }
+                wave_lds_sync();
+            }
+            if (lane < 16 && g0 + lane < m && acc > -FLT_MAX) keys[g0 + lane] = make_key(acc, (uint32_t)myrow);
+        }
+    } else {
+    const int R = p.xfmt ? HBD : BD;                 // rows per tile of the packed layout
     const size_t ks_stride = (size_t)R * 64;              // bytes between a row's consecutive K-stages
     for (int g0 = wave * 16; g0 < m; g0 += NW * 16) {
         const int r = lane >> 2, pc = lane & 3;
@@ -1068,7 +1134,7 @@ rescore_kernel(const RescoreParams p) {
                 const int nb = p.nks - ks0 < RS_KB ? p.nks - ks0 : RS_KB;
                 for (int u = 0; u < nb; ++u) {
                     const char* line = stage + (u * 16 + lane) * RS_ROW;
-                    if (!p.x_is_bf16) {
+                    if (!p.xfmt) {
                         const f32x4 c0 = *(const f32x4*)(line + ((0 ^ mysw) << 4)), c1 = *(const f32x4*)(line + ((1 ^ mysw) << 4));
                         const f32x4 c2 = *(const f32x4*)(line + ((2 ^ mysw) << 4)), c3 = *(const f32x4*)(line + ((3 ^ mysw) << 4));
                         const float* qq = qs + (ks0 + u) * 16;
@@ -1094,6 +1160,7 @@ rescore_kernel(const RescoreParams p) {
         }
         if (lane < 16 && g0 + lane < m && acc > -FLT_MAX)        // the fp32 scan's admission rule
             keys[g0 + lane] = make_key(acc, (uint32_t)myrow);
+    }
     }
     __syncthreads();
     const uint64_t* res = keys;

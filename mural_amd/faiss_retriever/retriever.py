@@ -12,7 +12,7 @@ import os
 import numpy as np
 from tqdm import tqdm
 
-from .. import _lib
+from .. import _lib, mx4
 
 logger = logging.getLogger(__name__)
 
@@ -37,7 +37,7 @@ class FlatIPIndex:
     coalesce_queries = 8192
 
     #: IPX_STORAGE / storage= values (include/ipx.h, ipx_set_param "storage")
-    STORAGE = {"f32": 0, "bf16scan": 1, "bf16": 2}
+    STORAGE = {"f32": 0, "bf16scan": 1, "bf16": 2, "mx4": 3}
 
     def __init__(self, d, device=None, storage=None):
         if device is None:
@@ -163,6 +163,89 @@ class FlatIPIndex:
                                                 A, int(bool(logits)), n, k, C.c_void_p(D.data_ptr()),
                                                 C.c_void_p(I.data_ptr()), 1, _torch_stream(aspect_emb)))
         return D, I
+
+    # ---- 4-bit rows (storage="mx4"), score matrices, stored rows by id ----
+    def add_mx4(self, codes, scales):
+        """Append rows that are in mx4 already (mural_amd.mx4.quantize): numpy arrays, or CUDA tensors on this index's GPU."""
+        L = _lib.lib()
+        if _is_torch_tensor(codes):
+            codes, scales = mx4.check_torch_pair(codes, scales, self.d, self.device)
+            _lib.check(L.ipx_add_mx4(self._h, C.c_void_p(codes.data_ptr()), C.c_void_p(scales.data_ptr()), codes.shape[0], 1,
+                                     _torch_stream(codes)))
+            return
+        codes, scales = mx4.check_numpy_pair(codes, scales, self.d)
+        _lib.check(L.ipx_add_mx4(self._h, C.c_void_p(codes.ctypes.data), C.c_void_p(scales.ctypes.data), codes.shape[0], 0, None))
+
+    def scores(self, q, start=0, n=None):
+        """The inner products of every query with rows start .. start + n - 1 (default: all to the end), fp32 [nq, n].
+        Needs storage="mx4". q: float32 / float16 (/ bfloat16, torch) [nq, d]; CUDA tensors give a CUDA tensor,
+        stream-ordered."""
+        L = _lib.lib()
+        nq, d = q.shape
+        assert d == self.d
+        n = self.ntotal - start if n is None else n
+        if _is_torch_tensor(q):
+            import torch
+            dt = {torch.float32: _lib.IPX_F32, torch.float16: _lib.IPX_F16, torch.bfloat16: _lib.IPX_BF16}[q.dtype]
+            assert q.is_cuda and q.device.index == self.device
+            q = q.contiguous()
+            out = torch.empty((nq, max(n, 0)), dtype=torch.float32, device=q.device)
+            _lib.check(L.ipx_scores(self._h, C.c_void_p(q.data_ptr()), dt, nq, start, n, C.c_void_p(out.data_ptr()), 1,
+                                    _torch_stream(q)))
+            return out
+        q = np.ascontiguousarray(q, dtype=q.dtype if q.dtype in _NP_DTYPES else "float32")
+        out = np.empty((nq, max(n, 0)), dtype=np.float32)
+        _lib.check(L.ipx_scores(self._h, C.c_void_p(q.ctypes.data), _NP_DTYPES[q.dtype], nq, start, n,
+                                C.c_void_p(out.ctypes.data), 0, None))
+        return out
+
+    def scores_mx4(self, codes, scales, start=0, n=None):
+        """`scores` with queries in mx4 (mural_amd.mx4.quantize): stored rows against stored rows, exact products."""
+        L = _lib.lib()
+        n = self.ntotal - start if n is None else n
+        if _is_torch_tensor(codes):
+            import torch
+            codes, scales = mx4.check_torch_pair(codes, scales, self.d, self.device)
+            out = torch.empty((codes.shape[0], max(n, 0)), dtype=torch.float32, device=codes.device)
+            _lib.check(L.ipx_scores_mx4(self._h, C.c_void_p(codes.data_ptr()), C.c_void_p(scales.data_ptr()), codes.shape[0],
+                                        start, n, C.c_void_p(out.data_ptr()), 1, _torch_stream(codes)))
+            return out
+        codes, scales = mx4.check_numpy_pair(codes, scales, self.d)
+        out = np.empty((codes.shape[0], max(n, 0)), dtype=np.float32)
+        _lib.check(L.ipx_scores_mx4(self._h, C.c_void_p(codes.ctypes.data), C.c_void_p(scales.ctypes.data), codes.shape[0],
+                                    start, n, C.c_void_p(out.ctypes.data), 0, None))
+        return out
+
+    def lookup(self, ids, scale=None, dtype=None):
+        """The stored rows with these ids (any shape, as `search` returns them; -1 gives a row of zeros), each times its
+        scale: [*ids.shape, d], float32 unless `dtype` says otherwise (torch: float32, float16, bfloat16; numpy: float32,
+        float16). Any storage. Numpy ids that are no rows of the index raise; CUDA ids that are not give zeros and the
+        next check() raises."""
+        L = _lib.lib()
+        if _is_torch_tensor(ids):
+            import torch
+            dtype = dtype or torch.float32
+            dt = {torch.float32: _lib.IPX_F32, torch.float16: _lib.IPX_F16, torch.bfloat16: _lib.IPX_BF16}[dtype]
+            assert ids.dtype == torch.int64 and ids.is_cuda and ids.device.index == self.device
+            ids = ids.contiguous()
+            if scale is not None:
+                assert scale.shape == ids.shape and scale.device == ids.device
+                scale = scale.contiguous().float()
+            out = torch.empty((*ids.shape, self.d), dtype=dtype, device=ids.device)
+            _lib.check(L.ipx_lookup(self._h, C.c_void_p(ids.data_ptr()), ids.numel(),
+                                    None if scale is None else C.c_void_p(scale.data_ptr()), C.c_void_p(out.data_ptr()), dt, 1,
+                                    _torch_stream(ids)))
+            return out
+        ids = np.ascontiguousarray(ids, dtype=np.int64)
+        if scale is not None:
+            scale = np.ascontiguousarray(scale, dtype=np.float32)
+            assert scale.shape == ids.shape
+        dtype = np.dtype(dtype or np.float32)
+        out = np.empty((*ids.shape, self.d), dtype=dtype)
+        _lib.check(L.ipx_lookup(self._h, C.c_void_p(ids.ctypes.data), ids.size,
+                                None if scale is None else C.c_void_p(scale.ctypes.data), C.c_void_p(out.ctypes.data),
+                                _NP_DTYPES[dtype], 0, None))
+        return out
 
     # ---- MURAL pooler on the device (MULGRAIN_Pooler.forward 'att', modeling/mul_grain.py:97-132) ----
     def _pool_args(self, hidden, weight, bias, begin_id):

@@ -1,0 +1,102 @@
+"""Rows in microscaled 4-bit floating point ("mx4"; include/ipx.h, ipx_mx4_quantize).
+
+32 consecutive elements of a row share a power-of-two scale, an element is one of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} times it:
+17 bytes per 32 elements. `quantize` gives the two arrays a service stores or ships (codes uint8 [n, nb, 16], scales uint8
+[n, nb], nb = ceil(d / 32)); FlatIPIndex(d, storage="mx4") takes them with add_mx4, or quantises rows itself in add.
+No counterpart in the reference.
+"""
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+
+BLOCK = 32
+
+
+def n_blocks(d):
+    return -(-int(d) // BLOCK)
+
+
+def _is_torch(x):
+    return type(x).__module__.startswith("torch") and hasattr(x, "data_ptr")
+
+
+def _torch_dtypes():
+    import torch
+    return {torch.float32: _lib.IPX_F32, torch.float16: _lib.IPX_F16, torch.bfloat16: _lib.IPX_BF16}
+
+
+def _torch_stream(x):
+    import torch
+    return C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)
+
+
+def check_torch_pair(codes, scales, d, device=None):
+    """(codes, scales) of n rows of d elements as CUDA tensors: shapes, types, one device. Returns them contiguous."""
+    import torch
+    nb = n_blocks(d)
+    assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8
+    assert codes.ndim == 3 and tuple(codes.shape[1:]) == (nb, 16) and tuple(scales.shape) == (codes.shape[0], nb)
+    assert codes.is_cuda and scales.device == codes.device
+    assert device is None or codes.device.index == device
+    return codes.contiguous(), scales.contiguous()
+
+
+def check_numpy_pair(codes, scales, d):
+    codes, scales = np.ascontiguousarray(codes), np.ascontiguousarray(scales)
+    nb = n_blocks(d)
+    assert codes.dtype == np.uint8 and scales.dtype == np.uint8
+    assert codes.ndim == 3 and codes.shape[1:] == (nb, 16) and scales.shape == (codes.shape[0], nb)
+    return codes, scales
+
+
+def quantize(x, device=0):
+    """x [n, d] -> (codes uint8 [n, nb, 16], scales uint8 [n, nb]). torch CUDA tensors (float32 / float16 / bfloat16; rows
+    may be a strided view with adjacent elements) give CUDA tensors on their device, stream-ordered; numpy arrays (float32 /
+    float16, anything else is converted to float32) give numpy arrays, computed on GPU `device`."""
+    L = _lib.lib()
+    if _is_torch(x):
+        import torch
+        n, d = x.shape
+        dt = _torch_dtypes()[x.dtype]
+        assert x.is_cuda
+        if d > 1 and x.stride(1) != 1 or n > 1 and x.stride(0) < d:
+            x = x.contiguous()
+        codes = torch.empty((n, n_blocks(d), 16), dtype=torch.uint8, device=x.device)
+        scales = torch.empty((n, n_blocks(d)), dtype=torch.uint8, device=x.device)
+        stride = x.stride(0) if n > 1 else d
+        _lib.check(L.ipx_mx4_quantize(C.c_void_p(x.data_ptr()), n, d, stride, dt, C.c_void_p(codes.data_ptr()),
+                                      C.c_void_p(scales.data_ptr()), 1, x.device.index, _torch_stream(x)))
+        return codes, scales
+    n, d = x.shape
+    x = np.ascontiguousarray(x, dtype=x.dtype if x.dtype in (np.float32, np.float16) else np.float32)
+    codes = np.empty((n, n_blocks(d), 16), dtype=np.uint8)
+    scales = np.empty((n, n_blocks(d)), dtype=np.uint8)
+    dt = _lib.IPX_F32 if x.dtype == np.float32 else _lib.IPX_F16
+    _lib.check(L.ipx_mx4_quantize(C.c_void_p(x.ctypes.data), n, d, d, dt, C.c_void_p(codes.ctypes.data),
+                                  C.c_void_p(scales.ctypes.data), 0, int(device), None))
+    return codes, scales
+
+
+def dequantize(codes, scales, d, dtype=None, device=0):
+    """The values [n, d] that (codes, scales) stand for, as float32 unless `dtype` says otherwise (torch: float32, float16,
+    bfloat16; numpy: float32, float16). Exact in float32 and bfloat16."""
+    L = _lib.lib()
+    d = int(d)
+    if _is_torch(codes):
+        import torch
+        dtype = dtype or torch.float32
+        dt = _torch_dtypes()[dtype]
+        codes, scales = check_torch_pair(codes, scales, d)
+        out = torch.empty((codes.shape[0], d), dtype=dtype, device=codes.device)
+        _lib.check(L.ipx_mx4_dequantize(C.c_void_p(codes.data_ptr()), C.c_void_p(scales.data_ptr()), codes.shape[0], d,
+                                        C.c_void_p(out.data_ptr()), dt, 1, codes.device.index, _torch_stream(codes)))
+        return out
+    dtype = np.dtype(dtype or np.float32)
+    dt = {np.dtype("float32"): _lib.IPX_F32, np.dtype("float16"): _lib.IPX_F16}[dtype]
+    codes, scales = check_numpy_pair(codes, scales, d)
+    out = np.empty((codes.shape[0], d), dtype=dtype)
+    _lib.check(L.ipx_mx4_dequantize(C.c_void_p(codes.ctypes.data), C.c_void_p(scales.ctypes.data), codes.shape[0], d,
+                                    C.c_void_p(out.ctypes.data), dt, 0, int(device), None))
+    return out
