@@ -314,8 +314,19 @@ int grow_corpus_x(ipx_index* ix, int64_t need_groups, hipStream_t st) {
     return 0;
 }
 
-// Division of a thread number by `by` on the device (div_by in ipx_mx4_kernels.h).
-uint64_t magic_of(uint64_t by) { return by <= 1 ? 0 : ~0ull / by + 1; }
+// Lanes per row of the mx4 row kernels, as a power of two: the most that leave at most a quarter of them idle, else those
+// that leave the fewest idle. np: pieces of eight elements per row.
+int mx4_lanes(int np, int least_l2) {
+    int best = least_l2;
+    double best_use = 0.0;
+    for (int l2 = 6; l2 >= least_l2; --l2) {
+        const int lanes = 1 << l2, turns = (np + lanes - 1) / lanes;
+        const double use = (double)np / ((double)turns * lanes);
+        if (use >= 0.75) return l2;
+        if (use > best_use) { best = l2; best_use = use; }
+    }
+    return best;
+}
 // A launch numbers its threads with 32 bits: rows per launch when a row takes `per_row` of them.
 int64_t rows_per_launch(int64_t per_row) { return std::max<int64_t>(1, (int64_t)(1ll << 31) / per_row); }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -326,17 +337,18 @@ int launch_mx4_quantize(const void* rows, int dtype, int64_t n, int d, int64_t s
     const int nb = (d + 31) / 32, np = nb * 4;
     const size_t el = dtype == IPX_F32 ? 4 : 2;
     const bool wide = aligned16(rows) && stride * el % 16 == 0;
-    const int64_t slice = rows_per_launch(np);
+    const int l2 = mx4_lanes(np, 2);
+    const int64_t slice = rows_per_launch(1 << l2);
     for (int64_t r0 = 0; r0 < n; r0 += slice) {
-        const uint32_t total = (uint32_t)(std::min(slice, n - r0) * np);
+        const uint32_t m = (uint32_t)std::min(slice, n - r0);
         const void* src = (const char*)rows + (size_t)r0 * stride * el;
-        const dim3 grid((total + 255) / 256), block(256);
+        const dim3 grid((unsigned)((((int64_t)m << l2) + 255) / 256)), block(256);
         if (ix)
-            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<true>, grid, block, 0, st, src, dtype, stride, total, magic_of(np), np, d,
-                               wide, ix->Xx, ix->Xxs, row0 + r0, ix->nks_x, ix->nkq_x);
+            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<true>, grid, block, 0, st, src, dtype, stride, m, l2, np, d, wide,
+                               ix->Xx, ix->Xxs, row0 + r0, ix->nks_x, ix->nkq_x);
         else
-            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<false>, grid, block, 0, st, src, dtype, stride, total, magic_of(np), np, d,
-                               wide, codes + (size_t)r0 * nb * 16, scales + (size_t)r0 * nb, (int64_t)0, 0, 0);
+            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<false>, grid, block, 0, st, src, dtype, stride, m, l2, np, d, wide,
+                               codes + (size_t)r0 * nb * 16, scales + (size_t)r0 * nb, (int64_t)0, 0, 0);
         IPX_HIP(hipGetLastError());
     }
     return 0;
@@ -436,20 +448,16 @@ int dtype_size(int dtype) { return dtype == IPX_F32 ? 4 : 2; }
 struct Geometry { int nqb, ntiles, S, R, G, cap; };
 
 // Deep lists: the splits' unsorted lists of every query (ScanParams::deepK / deepN) -> sorted top k_out (dD / dI).
-int launch_lists_finish(ipx_index* ix, const uint64_t* keys, const int* counts, int S, int k_list, int k_out, int64_t nq, float* dD,
-                        int64_t* dI, hipStream_t st) {
+int launch_deep_finish(ipx_index* ix, int S, int k_list, int k_out, int64_t nq, float* dD, int64_t* dI, hipStream_t st) {
     const int64_t total = (int64_t)S * k_list;
     const int P_max = (int)std::min<int64_t>(ipx::DEEP_LDS_KEYS, next_pow2((int)std::min<int64_t>(total, ipx::DEEP_LDS_KEYS)));
     const int lds = std::max(P_max, 2) * 8 + (S + 1) * 4 + 256 * 4;
     if (lds > 64 * 1024)
         IPX_HIP(hipFuncSetAttribute((const void*)ipx::deep_finish_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    hipLaunchKernelGGL(ipx::deep_finish_kernel, dim3((unsigned)nq), dim3(1024), lds, st, keys, counts, S, k_list, k_out, std::max(P_max, 2), ix->id_base, dD, dI);
+    hipLaunchKernelGGL(ipx::deep_finish_kernel, dim3((unsigned)nq), dim3(1024), lds, st, (const uint64_t*)ix->deepK.p,
+                       (const int*)ix->deepN.p, S, k_list, k_out, std::max(P_max, 2), ix->id_base, dD, dI);
     IPX_HIP(hipGetLastError());
     return 0;
-}
-
-int launch_deep_finish(ipx_index* ix, int S, int k_list, int k_out, int64_t nq, float* dD, int64_t* dI, hipStream_t st) {
-    return launch_lists_finish(ix, (const uint64_t*)ix->deepK.p, (const int*)ix->deepN.p, S, k_list, k_out, nq, dD, dI, st);
 }
 
 // ---- fp32 scan of a small batch (scan_f32_small_kernel: 32 or 64 queries per workgroup, two workgroups per CU):
@@ -784,7 +792,7 @@ int scan_f32_deep(ipx_index* ix, const float* dq, const float* dw, int A, int lo
 int launch_rescore(const ipx::RescoreParams& rp, int64_t nblocks, hipStream_t st) {
     const int dpad = rp.xfmt == 2 ? (rp.nks + 1) / 2 * 128 : rp.nks * (rp.xfmt ? 32 : 16);
     const int fixed = ((dpad * 4 + 15) & ~15) + rp.P * 8 + (rp.P <= ipx::RS_RANK_SORT ? rp.P * 8 : 0);
-    const int per_wave = ipx::RS_KB * 16 * ipx::RS_ROW;
+    const int per_wave = rp.xfmt == 2 ? 0 : ipx::RS_KB * 16 * ipx::RS_ROW;      // (mx4 rows are not staged)
     const int nw = (nblocks <= 128 && fixed + 16 * per_wave <= 160 * 1024) ? 16 : 4;
     const int rlds = fixed + nw * per_wave;
     void (*kern)(const ipx::RescoreParams) = rp.xfmt == 2 ? (nw == 16 ? ipx::rescore_kernel<16, true> : ipx::rescore_kernel<4, true>)
@@ -1348,26 +1356,22 @@ constexpr int MX_PARTS_SCORES = 5;       // ... in ipx_scores: as exact as fp32
 constexpr int MX_MAX_K = IPX_MAX_K;      // deepest list of a search
 constexpr int MX_SLICE = 4096;           // queries per pass of a search (bounds the workspace)
 
-// How a product runs: queries per workgroup, quads of the query block in LDS at a time, splits of the corpus.
-struct MxGeom { int cg, qc, nqb, S, lds; int64_t rounds; };
+// How a product runs: 32-query groups per workgroup, splits of the corpus, whether the query block stays in LDS.
+struct MxGeom { int cg, nqb, S, lds; bool resident; int64_t rounds; };
 MxGeom mx4_geometry(const ipx_index* ix, int64_t nq, int quad_bytes_per_cg, int64_t ntiles) {
     MxGeom g;
     const int room = 160 * 1024 - 1024, extra = 128;         // extra: hit counters, 4 bytes per query
-    // the largest block (more queries per row operand) whose queries stay in LDS; when not even 32 queries fit (long
+    // the larger block (half the row traffic per product) when its queries stay in LDS; when not even 32 do (long
     // vectors), the quads go through LDS in turn
-    g.cg = nq <= 32 ? 1 : nq <= 64 ? 2 : 4;
-    const int want = g.cg;
-    while (g.cg > 1 && ix->nkq_x * quad_bytes_per_cg * g.cg + extra * g.cg > room) g.cg /= 2;
-    if (ix->nkq_x * quad_bytes_per_cg * g.cg + extra * g.cg > room) {
-        g.cg = want;
-        while (quad_bytes_per_cg * g.cg + extra * g.cg > room) g.cg /= 2;
-    }
-    g.qc = std::min(ix->nkq_x, (room - extra * g.cg) / (quad_bytes_per_cg * g.cg));
-    g.lds = g.qc * quad_bytes_per_cg * g.cg + extra * g.cg;
-    const int per_cu = g.lds <= 80 * 1024 - 512 ? 2 : 1;
+    auto whole = [&](int cg) { return (ix->nkq_x * quad_bytes_per_cg + extra) * cg; };
+    g.cg = nq <= 32 || whole(2) > room ? 1 : 2;
+    g.resident = whole(g.cg) <= room;
+    if (!g.resident) g.cg = nq <= 32 ? 1 : 2;
+    g.lds = g.resident ? whole(g.cg) : (quad_bytes_per_cg + extra) * g.cg;
     g.nqb = (int)((nq + 32 * g.cg - 1) / (32 * g.cg));
-    const int64_t most = std::max<int64_t>(1, (ntiles + 7) / 8);       // 8 waves, a tile each
-    g.S = (int)std::min<int64_t>(std::max(1, per_cu * ix->num_cus / g.nqb), most);
+    // (a short corpus goes to as many CUs as it has tiles: a tile per wave of few workgroups leaves the matrix cores of the
+    // other CUs idle — 100k x 768, one query: 19 us on 98 CUs)
+    g.S = (int)std::min<int64_t>(std::max(1, ix->num_cus / g.nqb), std::max<int64_t>(1, ntiles));
     g.rounds = (ntiles + (int64_t)g.S * 8 - 1) / ((int64_t)g.S * 8);
     return g;
 }
@@ -1375,10 +1379,9 @@ MxGeom mx4_geometry(const ipx_index* ix, int64_t nq, int quad_bytes_per_cg, int6
 template <int PARTS, int FMT, int MODE>
 int launch_mx4_product(const MxGeom& g, ipx::MxParams p, hipStream_t st) {
     p.S = g.S;
-    p.qc = g.qc;
-    void (*kern)(const ipx::MxParams) = g.cg == 1 ? ipx::mx4_product_kernel<1, PARTS, FMT, MODE>
-                                        : g.cg == 2 ? ipx::mx4_product_kernel<2, PARTS, FMT, MODE>
-                                                    : ipx::mx4_product_kernel<4, PARTS, FMT, MODE>;
+    void (*kern)(const ipx::MxParams) =
+        g.resident ? (g.cg == 1 ? ipx::mx4_product_kernel<1, PARTS, FMT, MODE, true> : ipx::mx4_product_kernel<2, PARTS, FMT, MODE, true>)
+                   : (g.cg == 1 ? ipx::mx4_product_kernel<1, PARTS, FMT, MODE, false> : ipx::mx4_product_kernel<2, PARTS, FMT, MODE, false>);
     if (int rc = ensure_dynamic_lds((const void*)kern, std::max(g.lds, 64 * 1024 + 1))) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)(g.nqb * g.S)), dim3(ipx::MX_THREADS), g.lds, st, p);
     IPX_HIP(hipGetLastError());
@@ -1404,18 +1407,18 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     const bool timing = primary && ix->timing, direct = N <= ipx::MX_DIRECT;
     const int quad1 = PARTS * ipx::mx_part_bytes<FMT>(32);
     const MxGeom g = mx4_geometry(ix, nq, quad1, ntiles);
-    // expected hits per query and split: all rows, or the share of the index above the sample's j-th score. j: the
-    // wanted list's share of the sample, m, plus 5 standard deviations of it and a little for short lists — the list
-    // comes out too short (the query is then repeated) with a probability below 1e-7.
-    constexpr int m_rows = ipx::MX_SAMPLE;
+    // The sample: more rows, hence a tighter floor and fewer hits, where the scores of the sample are few.
+    const int m_rows = nq <= 64 && N > 2 * ipx::MX_SAMPLE_FEW ? ipx::MX_SAMPLE_FEW : ipx::MX_SAMPLE_MANY;
+    // j: the wanted list's share of the sample, plus 4 standard deviations of it and a little for short lists — the list
+    // comes out too short (the query is then repeated) with a probability of about 1e-5.
     const double share = (double)kc * m_rows / (double)N;
-    const int j = (int)std::min<double>(m_rows, ceil(share + 5.0 * sqrt(share) + 6.0));
-    const double hits = (double)j * (double)N / m_rows / g.S;
-    // Room per query and split: half as much again and 10 standard deviations; at least one round's rows of a workgroup,
-    // all of which are hits where every score is equal (a zero query: the first rows of the index).
-    const int64_t round_rows = 8 * ipx::MX_TILE;
-    const int64_t cap = direct ? g.rounds * round_rows
-                               : std::min<int64_t>(g.rounds * round_rows, std::max<int64_t>(round_rows, ((int64_t)(1.5 * hits + 10.0 * sqrt(hits)) + 32) / 8 * 8));
+    const int j = (int)std::min<double>(m_rows, ceil(share + 4.0 * sqrt(share) + 4.0));
+    // Room per query and split: the expected hits, half as much again and 10 standard deviations; and, as all scores may be
+    // equal (a zero query: the first rows of the index are the hits), the rows of whole tiles dealt in turn.
+    const double hits = (double)j * (double)N / m_rows;
+    const int64_t split_rows = (ntiles + g.S - 1) / g.S * ipx::MX_TILE, turn_rows = ((int64_t)(hits / ipx::MX_TILE / g.S) + 2) * ipx::MX_TILE;
+    const int64_t cap = direct ? split_rows
+                               : std::min<int64_t>(split_rows, std::max<int64_t>(turn_rows, (int64_t)(1.5 * hits / g.S + 10.0 * sqrt(hits / g.S)) + 32));
     const size_t info_bytes = ((size_t)nq * sizeof(ipx::MxQueryInfo) + 255) / 256 * 256, word = ((size_t)nq * 4 + 255) / 256 * 256;
 
     if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
@@ -1423,14 +1426,14 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     if (int rc = ix->deepN.ensure((size_t)nq * g.S * sizeof(int))) return rc;
     if (int rc = ix->candD.ensure((size_t)nq * kc * sizeof(float))) return rc;
     if (int rc = ix->candI.ensure((size_t)nq * kc * sizeof(int64_t))) return rc;
-    if (int rc = ix->mxq.ensure(info_bytes + 4 * word)) return rc;         // norms, row bounds, floors, list states
+    if (int rc = ix->mxq.ensure(info_bytes + 3 * word)) return rc;         // norms, row bounds, floors, list states
     if (!direct)
         if (int rc = ix->mxs.ensure((size_t)nq * m_rows * sizeof(float))) return rc;
     if (int rc = ensure_hflags(ix, nq, st)) return rc;
     ipx::MxQueryInfo* info = (ipx::MxQueryInfo*)ix->mxq.p;
-    int64_t* below = (int64_t*)((char*)ix->mxq.p + info_bytes);
-    float* tau = (float*)((char*)ix->mxq.p + info_bytes + 2 * word);
-    int* todo = (int*)((char*)ix->mxq.p + info_bytes + 3 * word);
+    uint32_t* below = (uint32_t*)((char*)ix->mxq.p + info_bytes);
+    float* tau = (float*)((char*)ix->mxq.p + info_bytes + word);
+    int* todo = (int*)((char*)ix->mxq.p + info_bytes + 2 * word);
 
     if (timing) IPX_HIP(hipEventRecord(ix->ev[0], st));
     hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)(g.nqb * 32 * g.cg)), dim3(256), 0, st, (const void*)qf,
@@ -1448,15 +1451,16 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     } else {
         ipx::MxParams ps = p;
         ps.ntiles = m_rows / ipx::MX_TILE;
-        ps.gstep = (N / ipx::MX_GROUP - 2) / (ps.ntiles - 1);      // whole groups, spread over the index
+        ps.gstep = (N / ipx::MX_GROUP - ipx::MX_RG) / (ps.ntiles - 1);      // whole groups, spread over the index
         ps.out = (float*)ix->mxs.p;
         ps.ld = m_rows;
         ps.row0 = -1;
         ps.n = m_rows;
         MxGeom gs = g;
-        gs.S = (int)std::min<int64_t>(g.S, ps.ntiles / 8);
+        gs.S = (int)std::min<int64_t>(g.S, ps.ntiles);
         if (int rc = launch_mx4_product<PARTS, FMT, ipx::MX_SCORES>(gs, ps, st)) return rc;
-        hipLaunchKernelGGL(ipx::mx4_floor_kernel, dim3((unsigned)nq), dim3(1024), 0, st, (const float*)ix->mxs.p, m_rows, j, N, tau, below);
+        hipLaunchKernelGGL((m_rows == ipx::MX_SAMPLE_FEW ? ipx::mx4_floor_kernel<ipx::MX_SAMPLE_FEW / 1024> : ipx::mx4_floor_kernel<ipx::MX_SAMPLE_MANY / 1024>),
+                           dim3((unsigned)nq), dim3(1024), 0, st, (const float*)ix->mxs.p, j, N, tau, below);
         IPX_HIP(hipGetLastError());
     }
     if (timing) IPX_HIP(hipEventRecord(ix->ev[1], st));
@@ -1470,9 +1474,12 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     p.cap = (int)cap;
     if (int rc = launch_mx4_product<PARTS, FMT, ipx::MX_SEARCH>(g, p, st)) return rc;
     if (timing) IPX_HIP(hipEventRecord(ix->ev[2], st));
-    if (int rc = launch_lists_finish(ix, (const uint64_t*)ix->cand.p, (const int*)ix->deepN.p, g.S, (int)cap, kc, nq,
-                                     (float*)ix->candD.p, (int64_t*)ix->candI.p, st))
-        return rc;
+    const int Pmax = next_pow2(std::max(512, kc + kc / 4));
+    const int slds = (Pmax + ipx::MX_HELD) * 8 + g.S * 4;
+    if (int rc = ensure_dynamic_lds((const void*)ipx::mx4_select_kernel, std::max(slds, 64 * 1024 + 1))) return rc;
+    hipLaunchKernelGGL(ipx::mx4_select_kernel, dim3((unsigned)nq), dim3(1024), slds, st, (const uint64_t*)ix->cand.p,
+                       (const int*)ix->deepN.p, g.S, (int)cap, kc, Pmax, ix->id_base, (float*)ix->candD.p, (int64_t*)ix->candI.p);
+    IPX_HIP(hipGetLastError());
     if (timing) {
         IPX_HIP(hipEventRecord(ix->ev[3], st));
         ix->ev_merge = true;
@@ -1955,7 +1962,7 @@ int ipx_add_mx4(ipx_index* ix, const uint8_t* codes, const uint8_t* scales, int6
             s = c + cb;
         }
         const uint32_t total = (uint32_t)(m * nb);
-        hipLaunchKernelGGL(ipx::mx4_place_kernel, dim3((total + 255) / 256), dim3(256), 0, st, c, s, total, magic_of(nb), nb, ix->d,
+        hipLaunchKernelGGL(ipx::mx4_place_kernel, dim3((total + 255) / 256), dim3(256), 0, st, c, s, total, nb, ix->d,
                            ix->Xx, ix->Xxs, ix->ntotal + r0, ix->nks_x, ix->nkq_x);
         IPX_HIP(hipGetLastError());
     }
@@ -2039,11 +2046,13 @@ int ipx_lookup(ipx_index* ix, const int64_t* ids, int64_t n, const float* scale,
     const void* X = xfmt == 2 ? (const void*)ix->Xx : xfmt ? (const void*)ix->Xh : (const void*)ix->Xp;
     const int nks = xfmt == 2 ? ix->nks_x : xfmt ? ix->nks_h : ix->nks;
     const bool wide = aligned16(dout) && row_bytes % 16 == 0;
-    const int64_t slice = rows_per_launch(np);
+    const int l2 = mx4_lanes(np, 0);
+    const int64_t slice = rows_per_launch(1 << l2);
+    auto kern = xfmt == 2 ? ipx::lookup_kernel<2> : xfmt == 1 ? ipx::lookup_kernel<1> : ipx::lookup_kernel<0>;
     for (int64_t i0 = 0; i0 < n; i0 += slice) {
-        const uint32_t total = (uint32_t)(std::min(slice, n - i0) * np);
-        hipLaunchKernelGGL(ipx::lookup_kernel, dim3((total + 255) / 256), dim3(256), 0, st, X, (const uint8_t*)ix->Xxs, xfmt, nks,
-                           ix->nkq_x, ix->id_base, ix->ntotal, di + i0, ds ? ds + i0 : nullptr, total, magic_of(np), np, d,
+        const uint32_t m = (uint32_t)std::min(slice, n - i0);
+        hipLaunchKernelGGL(kern, dim3((unsigned)((((int64_t)m << l2) + 255) / 256)), dim3(256), 0, st, X, (const uint8_t*)ix->Xxs, nks,
+                           ix->nkq_x, ix->id_base, ix->ntotal, di + i0, ds ? ds + i0 : nullptr, m, l2, np, d,
                            (void*)(dout + (size_t)i0 * row_bytes), dtype, wide, (int*)ix->err.p + LOOKUP_ERR);
         IPX_HIP(hipGetLastError());
     }
@@ -2113,11 +2122,12 @@ int ipx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n, i
     const int np = (d + 7) / 8;
     // (the wide form also reads the codes as dwords: they then start at a multiple of 4 bytes)
     const bool wide = aligned16(dout) && row_bytes % 16 == 0 && ((uintptr_t)dc & 3) == 0;
-    const int64_t slice = rows_per_launch(np);
+    const int l2 = mx4_lanes(np, 0);
+    const int64_t slice = rows_per_launch(1 << l2);
     for (int64_t r0 = 0; r0 < n && e == hipSuccess; r0 += slice) {
-        const uint32_t total = (uint32_t)(std::min(slice, n - r0) * np);
-        hipLaunchKernelGGL(ipx::mx4_dequantize_kernel, dim3((total + 255) / 256), dim3(256), 0, st, dc + (size_t)r0 * nb * 16,
-                           ds + (size_t)r0 * nb, total, magic_of(np), np, d, (int)nb, (void*)(dout + (size_t)r0 * row_bytes), dtype, wide);
+        const uint32_t m = (uint32_t)std::min(slice, n - r0);
+        hipLaunchKernelGGL(ipx::mx4_dequantize_kernel, dim3((unsigned)((((int64_t)m << l2) + 255) / 256)), dim3(256), 0, st,
+                           dc + (size_t)r0 * nb * 16, ds + (size_t)r0 * nb, m, l2, np, d, (int)nb, (void*)(dout + (size_t)r0 * row_bytes), dtype, wide);
         e = hipGetLastError();
     }
     if (!on_device) {

@@ -1051,55 +1051,57 @@ rescore_kernel(const RescoreParams p) {
     uint64_t* sorted = keys + p.P;                            // [P] when by_rank
     char* stage = (char*)(sorted + (by_rank ? p.P : 0)) + wave * (RS_KB * 16 * RS_ROW);
     if constexpr (MX4) {
-        // The same with mx4 rows: a line is 128 elements (two K-sets), four blocks of 16 bytes; lane r < 16 also loads its
-        // row's scales, four dwords a round. A block's values are codes times a power of two: exact, so the chain is the
-        // one a bf16 index of these values runs.
+        // mx4 rows: 64 candidates per wave, one per lane — the chain of a candidate is serial, so the lanes are what there is
+        // to fill (four lanes to a row and 16 chains a wave took 360 us for 1000 x 1500 candidates of 768). A lane fetches
+        // its own row, 64 bytes (128 elements, two K-sets) at a time, one line ahead, and its scales, one quad ahead. Values
+        // are exact in fp32, so the chain is the one a bf16 index of these values runs.
         const int nb = (p.d + 31) / 32, nlines = (p.nks + 1) / 2;
-        for (int g0 = wave * 16; g0 < m; g0 += NW * 16) {
-            const int r = lane >> 2, pc = lane & 3;
-            const int64_t row = cI[g0 + r < m ? g0 + r : m - 1] - p.id_base;
-            const char* src = (const char*)p.X + (size_t)(row >> 5) * p.nks * 1024 + (row & 31) * 32 + (pc & 1) * 16;
+        for (int g0 = wave * 64; g0 < m; g0 += NT) {
             const int my = g0 + lane < m ? g0 + lane : m - 1;
-            const int64_t myrow = lane < 16 ? cI[my] - p.id_base : 0;
-            const uint32_t* sp = (const uint32_t*)(p.Xs + (size_t)myrow * p.nkq * 8);
+            const int64_t row = cI[my] - p.id_base;
+            const uint8_t* src = (const uint8_t*)p.X + (size_t)(row >> 5) * p.nks * 1024;
+            const int rr = (int)(row & 31);
+            const uint2* sp = (const uint2*)(p.Xs + (size_t)row * p.nkq * 8);
             float acc = 0.f;
-            const int last = p.nks - 1;
-            auto fetch = [&](int line) { const int ks = 2 * line + (pc >> 1); return *(const uint4*)(src + (size_t)(ks < last ? ks : last) * 1024); };
-            auto scales = [&](int i) { return lane < 16 ? sp[i < 2 * p.nkq ? i : 2 * p.nkq - 1] : 0u; };
-            uint4 v0 = fetch(0), v1 = fetch(1), v2 = fetch(2), v3 = fetch(3);
-            uint32_t s0 = scales(0), s1 = scales(1), s2 = scales(2), s3 = scales(3);
-            for (int l0 = 0; l0 < nlines; l0 += 4) {
-                *(uint4*)(stage + (0 * 16 + r) * RS_ROW + pc * 16) = v0;
-                *(uint4*)(stage + (1 * 16 + r) * RS_ROW + pc * 16) = v1;
-                *(uint4*)(stage + (2 * 16 + r) * RS_ROW + pc * 16) = v2;
-                *(uint4*)(stage + (3 * 16 + r) * RS_ROW + pc * 16) = v3;
-                const uint32_t c0 = s0, c1 = s1, c2 = s2, c3 = s3;
-                v0 = fetch(l0 + 4); v1 = fetch(l0 + 5); v2 = fetch(l0 + 6); v3 = fetch(l0 + 7);
-                s0 = scales(l0 + 4); s1 = scales(l0 + 5); s2 = scales(l0 + 6); s3 = scales(l0 + 7);
-                wave_lds_sync();
-                if (lane < 16) {
-                    const int blocks = nb - l0 * 4 < 16 ? nb - l0 * 4 : 16;
-                    for (int b = 0; b < blocks; ++b) {             // block b: K-set b >> 1, half b & 1
-                        const uint32_t word = b & 8 ? (b & 1 ? c3 : c2) : (b & 1 ? c1 : c0);
-                        const uint32_t byte = (word >> (8 * ((b >> 1) & 3))) & 255u;
-                        const float sc = __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
-                        const uint4 w = *(const uint4*)(stage + ((b >> 2) * 16 + lane) * RS_ROW + (b & 3) * 16);
-                        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+            uint4 v[4];
+            // (ipx_mx4_kernels.h, mx_code_at: a last K-set without a partner lies in 32-byte pieces; its line is read twice
+            // over, the second half is not used)
+            auto fetch = [&](int line) {
+                line = line < nlines ? line : nlines - 1;
+                const bool alone = 2 * line + 1 == p.nks;
+                const uint4* at = (const uint4*)(src + line * 2048 + (alone ? rr * 32 : rr * 64));
+                v[0] = at[0];
+                v[1] = at[1];
+                v[2] = at[alone ? 0 : 2];
+                v[3] = at[alone ? 1 : 3];
+            };
+            fetch(0);
+            uint2 sc = sp[0];
+            for (int line = 0; line < nlines; ++line) {
+                const uint4 c[4] = {v[0], v[1], v[2], v[3]};
+                const uint32_t two = (line & 1) * 16;                       // this line's scale bytes of the quad
+                const uint32_t s0 = sc.x >> two, s1 = sc.y >> two;
+                fetch(line + 1);
+                if (line & 1) sc = sp[(line + 1) / 2 < p.nkq ? (line + 1) / 2 : p.nkq - 1];
+                const int blocks = nb - line * 4;                           // 4 except in the last line
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float* qq = qs + (l0 * 4 + b) * 32 + i * 8;
-                            const auto e01 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], 1.f, 0), e23 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], 1.f, 1);
-                            const auto e45 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], 1.f, 2), e67 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], 1.f, 3);
-                            acc = fmaf(e01[0] * sc, qq[0], acc); acc = fmaf(e45[0] * sc, qq[4], acc);
-                            acc = fmaf(e01[1] * sc, qq[1], acc); acc = fmaf(e45[1] * sc, qq[5], acc);
-                            acc = fmaf(e23[0] * sc, qq[2], acc); acc = fmaf(e67[0] * sc, qq[6], acc);
-                            acc = fmaf(e23[1] * sc, qq[3], acc); acc = fmaf(e67[1] * sc, qq[7], acc);
-                        }
+                for (int b = 0; b < 4; ++b) {                               // block b: K-set b >> 1, half b & 1
+                    if (b >= blocks) break;
+                    const float s = __uint_as_float((((b & 1) ? s1 : s0) >> (8 * (b >> 1)) & 255u) << 23);
+                    const uint32_t ws[4] = {c[b].x, c[b].y, c[b].z, c[b].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 qa = *(const f32x4*)(qs + (line * 4 + b) * 32 + i * 8), qb = *(const f32x4*)(qs + (line * 4 + b) * 32 + i * 8 + 4);
+                        const auto e01 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], s, 0), e23 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], s, 1);
+                        const auto e45 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], s, 2), e67 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(ws[i], s, 3);
+                        acc = fmaf(e01[0], qa[0], acc); acc = fmaf(e45[0], qb[0], acc);
+                        acc = fmaf(e01[1], qa[1], acc); acc = fmaf(e45[1], qb[1], acc);
+                        acc = fmaf(e23[0], qa[2], acc); acc = fmaf(e67[0], qb[2], acc);
+                        acc = fmaf(e23[1], qa[3], acc); acc = fmaf(e67[1], qb[3], acc);
                     }
                 }
-                wave_lds_sync();
             }
-            if (lane < 16 && g0 + lane < m && acc > -FLT_MAX) keys[g0 + lane] = make_key(acc, (uint32_t)myrow);
+            if (g0 + lane < m && acc > -FLT_MAX) keys[g0 + lane] = make_key(acc, (uint32_t)row);
         }
     } else {
     const int R = p.xfmt ? HBD : BD;                 // rows per tile of the packed layout

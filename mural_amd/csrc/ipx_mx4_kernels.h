@@ -13,8 +13,10 @@
 // In the index the same bytes lie as the scaled MFMA wants them. v_mfma_scale_f32_32x32x64_f8f6f4 multiplies 32 rows by
 // 32 columns over 64 elements: lane l holds row l & 31, elements 32 (l >> 5) .. + 31 — one whole block, 16 bytes, with
 // one scale. So a K-set is 64 elements (two blocks) and
-//   codes  [group of 32 rows][K-set][row][half][16 bytes]          one operand = one 1-KiB wave load
-//   scales [group of 32 rows][row][quad of 4 K-sets][half][4 bytes]  one dword = the scales of a lane's next four operands
+//   codes  [group of 32 rows][pair of K-sets][row][K-set of the pair][half][16 bytes]   (a last K-set without a partner:
+//          [row][half][16 bytes]): the two wave loads of a pair cover 2 KiB without a gap, and a single row is found in
+//          whole 64-byte pieces (rescoring and lookup gather rows; 32-byte pieces cost twice the traffic there)
+//   scales [row][quad of 4 K-sets][half][4 bytes]   one dword = the scales of a lane's next four operands
 // Rows go from HBM straight into the registers of the one wave that multiplies them; LDS holds the queries only.
 //
 // Queries. The matrix core takes its two operands in different formats; fp32 queries are split into E2M3 parts (sign, two
@@ -34,138 +36,144 @@ constexpr int MX_GROUP = 32;             // rows per group
 constexpr int MX_KSET = 64;              // elements per K-set
 constexpr int MX_SET_BYTES = 1024;       // codes of one K-set of one group
 constexpr int MX_THREADS = 512;          // 8 waves
-constexpr int MX_RG = 2;                 // groups per wave tile
+constexpr int MX_RG = 4;                 // groups per wave tile
 constexpr int MX_TILE = MX_RG * MX_GROUP;
-constexpr int MX_SAMPLE = 8192;          // rows a search samples for its floor (mx4_floor_kernel)
-constexpr int MX_DIRECT = 16384;         // indexes of up to this many rows are searched without a floor
+constexpr int MX_SAMPLE_FEW = 32768;     // rows a search samples for its floor: few queries (mx4_floor_kernel)
+constexpr int MX_SAMPLE_MANY = 8192;     // ... many
+constexpr int MX_DIRECT = 16384;         // indexes of up to this many rows are searched without a floor (fewer than the sample: neither)
 
 __device__ __forceinline__ float mx_scale_f32(uint32_t byte) {          // 2^(byte - 127); 255: NaN
     return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
 }
+// The conversions of the instruction set take the scale as the exponent field of a float: the scale byte itself, 0 and 255
+// (NaN) included.
+__device__ __forceinline__ float mx_scale_field(uint32_t byte) { return __uint_as_float(byte << 23); }
 // scale byte of a block from the largest magnitude's bits (sign cleared; NaN and inf order above all finite values)
 __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
     const uint32_t e = top >> 23;
     return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
 }
-__device__ __forceinline__ uint32_t mx_code(float x, float inv) {       // E2M1 code of x * inv
-    const float a = fabsf(x) * inv;
-    // steps of 0.5 below 2, of 1 below 4, of 2 beyond: the codes count the steps
-    const float c = a < 2.f ? rintf(a * 2.f) : a < 4.f ? rintf(a) + 2.f : fminf(rintf(a * 0.5f) + 4.f, 7.f);
-    return (uint32_t)(int)c | (__float_as_uint(x) >> 31 << 3);
+// eight values -> their codes under the scale; rounds to nearest, ties to even, and saturates
+__device__ __forceinline__ uint32_t mx_encode8(const float (&x)[8], uint32_t byte) {
+    const float s = mx_scale_field(byte);
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+    return byte == 255 ? 0u : w;
 }
-// eight codes of one dword -> values before scaling, elements in order
-__device__ __forceinline__ void mx_decode8(uint32_t w, float (&v)[8]) {
-    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
-    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
+// eight codes of one dword -> values, elements in order
+__device__ __forceinline__ void mx_decode8(uint32_t w, uint32_t byte, float (&v)[8]) {
+    const float s = mx_scale_field(byte);
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
     v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1]; v[4] = c[0]; v[5] = c[1]; v[6] = e[0]; v[7] = e[1];
 }
-// gid / np for gid < 2^32, 2 <= np < 2^32, magic = ceil(2^64 / np)
-__device__ __forceinline__ uint32_t div_by(uint32_t gid, uint64_t magic) { return (uint32_t)__umul64hi((uint64_t)gid, magic); }
 
 // where block b (32 elements) of row `row` lies in the index
 __device__ __forceinline__ size_t mx_code_at(int64_t row, int b, int nks) {
-    return ((size_t)(row >> 5) * nks + (b >> 1)) * MX_SET_BYTES + (row & 31) * 32 + (b & 1) * 16;
+    const int r = (int)(row & 31);
+    const bool alone = (nks & 1) && (b >> 2) == (nks >> 1);
+    return (size_t)(row >> 5) * nks * MX_SET_BYTES + (b >> 2) * 2 * MX_SET_BYTES + (alone ? r * 32 + (b & 1) * 16 : r * 64 + (b & 3) * 16);
 }
 __device__ __forceinline__ size_t mx_scale_at(int64_t row, int b, int nkq) {
     return (((size_t)row * nkq + (b >> 3)) * 2 + (b & 1)) * 4 + ((b >> 1) & 3);
 }
 
-__device__ __forceinline__ void store_as(void* out, int dtype, size_t i, float v) {
-    if (dtype == 0) ((float*)out)[i] = v;
-    else if (dtype == 1) ((__half*)out)[i] = __float2half_rn(v);
-    else ((uint16_t*)out)[i] = f32_to_bf16_rne(v);
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack2_as(int dtype, float lo, float hi) {      // two 16-bit values, rounded to nearest even
+    if (dtype == 1) return __builtin_bit_cast(uint32_t, f16x2{(_Float16)lo, (_Float16)hi});
+    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
 }
-// eight outputs; `wide`: they start at a multiple of 16 bytes
+// `count` of eight outputs from element i on; `wide`: they start at a multiple of 16 bytes
 __device__ __forceinline__ void store8(void* out, int dtype, size_t i, const float (&v)[8], int count, bool wide) {
-    if (wide && count == 8) {
+    if (wide && count >= 8) {
         if (dtype == 0) {
             float4* o = (float4*)((float*)out + i);
             o[0] = make_float4(v[0], v[1], v[2], v[3]);
             o[1] = make_float4(v[4], v[5], v[6], v[7]);
         } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint32_t lo, hi;
-                if (dtype == 1) {
-                    lo = __half_as_ushort(__float2half_rn(v[2 * e]));
-                    hi = __half_as_ushort(__float2half_rn(v[2 * e + 1]));
-                } else {
-                    lo = f32_to_bf16_rne(v[2 * e]);
-                    hi = f32_to_bf16_rne(v[2 * e + 1]);
-                }
-                w[e] = lo | hi << 16;
-            }
-            *(uint4*)((uint16_t*)out + i) = make_uint4(w[0], w[1], w[2], w[3]);
+            *(uint4*)((uint16_t*)out + i) = make_uint4(pack2_as(dtype, v[0], v[1]), pack2_as(dtype, v[2], v[3]),
+                                                       pack2_as(dtype, v[4], v[5]), pack2_as(dtype, v[6], v[7]));
         }
         return;
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-        if (e < count) store_as(out, dtype, i + e, v[e]);
+        if (e < count) {
+            if (dtype == 0) ((float*)out)[i + e] = v[e];
+            else ((uint16_t*)out)[i + e] = (uint16_t)pack2_as(dtype, v[e], 0.f);
+        }
 }
+
+// The row kernels below give a row 2^l2 adjacent lanes, each of which takes every 2^l2-th piece of eight elements; the host
+// picks the l2 that leaves the fewest lanes idle (mx4_lanes).
 
 // ---- quantisation ----------------------------------------------------------------------------------------------
 // Rows [n, d] (f32 / f16 / bf16, `stride` elements apart) -> codes and scales, in the external form or (INDEX) at rows
-// row0.. of an index. Four adjacent lanes per block, eight elements each: the block's largest magnitude is two exchanges
-// of lanes away, a wave reads 512 consecutive elements and writes 256 consecutive bytes. Bound by HBM.
+// row0.. of an index. Four adjacent lanes per block, eight elements each (2^l2 >= 4): the block's largest magnitude is two
+// exchanges of lanes away. Bound by HBM.
 template <bool INDEX>
 __global__ void __launch_bounds__(256)
-mx4_quantize_kernel(const void* __restrict__ src, int dtype, int64_t stride, uint32_t total, uint64_t magic, int np, int d,
-                    bool wide, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t row0, int nks, int nkq) {
-    const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
-    if (gid >= total) return;                               // a multiple of 4: the four lanes of a block stay together
-    const uint32_t r = div_by(gid, magic);
-    const int piece = (int)(gid - r * (uint32_t)np), e0 = piece * 8;
-    const int64_t at = (int64_t)r * stride + e0;
-    float x[8];
-    if (wide && e0 + 8 <= d) {
-        if (dtype == 0) {
-            const float4 a = *(const float4*)((const float*)src + at), b = *(const float4*)((const float*)src + at + 4);
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        } else {
-            const uint4 w = *(const uint4*)((const uint16_t*)src + at);
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+mx4_quantize_kernel(const void* __restrict__ src, int dtype, int64_t stride, uint32_t n, int l2, int np, int d, bool wide,
+                    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t row0, int nks, int nkq) {
+    const uint32_t gid = blockIdx.x * 256u + threadIdx.x, r = gid >> l2;
+    if (r >= n) return;
+    for (int piece = (int)(gid & ((1u << l2) - 1)); piece < np; piece += 1 << l2) {
+        const int e0 = piece * 8;
+        const int64_t at = (int64_t)r * stride + e0;
+        float x[8];
+        if (wide && e0 + 8 <= d) {
+            if (dtype == 0) {
+                const float4 a = *(const float4*)((const float*)src + at), b = *(const float4*)((const float*)src + at + 4);
+                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+            } else {
+                const uint4 w = *(const uint4*)((const uint16_t*)src + at);
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint16_t u = (uint16_t)(ws[e >> 1] >> (16 * (e & 1)));
-                x[e] = dtype == 1 ? __half2float(__ushort_as_half(u)) : __uint_as_float((uint32_t)u << 16);
+                for (int e = 0; e < 4; ++e) {
+                    if (dtype == 1) {
+                        const f16x2 v = __builtin_bit_cast(f16x2, ws[e]);
+                        x[2 * e] = (float)v[0];
+                        x[2 * e + 1] = (float)v[1];
+                    } else {
+                        x[2 * e] = bf16_lo(ws[e]);
+                        x[2 * e + 1] = bf16_hi(ws[e]);
+                    }
+                }
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = e0 + e < d ? load_as_f32(src, dtype, at + e) : 0.f;
         }
-    } else {
+        uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = e0 + e < d ? load_as_f32(src, dtype, at + e) : 0.f;
-    }
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));      // quad_perm [1,0,3,2]
-    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));      // quad_perm [2,3,0,1]
-    const uint32_t byte = mx_scale_byte(top);
-    const float inv = __uint_as_float((254u - byte) << 23);
-    uint32_t w = 0;
-    if (byte != 255)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w |= mx_code(x[e], inv) << (4 * e);
-    const int b = piece >> 2, p = piece & 3;
-    if constexpr (INDEX) {
-        const int64_t row = row0 + r;
-        *(uint32_t*)(codes + mx_code_at(row, b, nks) + p * 4) = w;
-        if (p == 0) scales[mx_scale_at(row, b, nkq)] = (uint8_t)byte;
-    } else {
-        const size_t blk = (size_t)r * (np >> 2) + b;
-        *(uint32_t*)(codes + blk * 16 + p * 4) = w;
-        if (p == 0) scales[blk] = (uint8_t)byte;
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));      // quad_perm [1,0,3,2]
+        top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));      // quad_perm [2,3,0,1]
+        const uint32_t byte = mx_scale_byte(top), w = mx_encode8(x, byte);
+        const int b = piece >> 2, p = piece & 3;
+        if constexpr (INDEX) {
+            const int64_t row = row0 + r;
+            *(uint32_t*)(codes + mx_code_at(row, b, nks) + p * 4) = w;
+            if (p == 0) scales[mx_scale_at(row, b, nkq)] = (uint8_t)byte;
+        } else {
+            const size_t blk = (size_t)r * (np >> 2) + b;
+            *(uint32_t*)(codes + blk * 16 + p * 4) = w;
+            if (p == 0) scales[blk] = (uint8_t)byte;
+        }
     }
 }
 
 // external form -> rows row0.. of an index; one thread per block
 __global__ void __launch_bounds__(256)
-mx4_place_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t total, uint64_t magic, int nb,
-                 int d, uint8_t* __restrict__ X, uint8_t* __restrict__ Xs, int64_t row0, int nks, int nkq) {
+mx4_place_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t total, int nb, int d,
+                 uint8_t* __restrict__ X, uint8_t* __restrict__ Xs, int64_t row0, int nks, int nkq) {
     const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
     if (gid >= total) return;
-    const uint32_t r = nb == 1 ? gid : div_by(gid, magic);
+    const uint32_t r = gid / (uint32_t)nb;
     const int b = (int)(gid - r * (uint32_t)nb);
     uint32_t w[4];
 #pragma unroll
@@ -179,24 +187,20 @@ mx4_place_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ 
     Xs[mx_scale_at(row0 + r, b, nkq)] = scales[gid];
 }
 
-// external form -> values; one thread per eight elements
+// external form -> values
 __global__ void __launch_bounds__(256)
-mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t total, uint64_t magic,
-                      int np, int d, int nb, void* __restrict__ out, int dtype, bool wide) {
-    const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
-    if (gid >= total) return;
-    const uint32_t r = np == 1 ? gid : div_by(gid, magic);
-    const int piece = (int)(gid - r * (uint32_t)np);
-    const size_t blk = (size_t)r * nb + (piece >> 2);
-    const uint8_t* s = codes + blk * 16 + (piece & 3) * 4;
-    const uint32_t w = wide ? *(const uint32_t*)s : s[0] | (uint32_t)s[1] << 8 | (uint32_t)s[2] << 16 | (uint32_t)s[3] << 24;
-    const float sc = mx_scale_f32(scales[blk]);
-    float v[8];
-    mx_decode8(w, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= sc;
-    const int left = d - piece * 8;
-    store8(out, dtype, (size_t)r * d + piece * 8, v, left < 8 ? left : 8, wide);
+mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t n, int l2, int np, int d, int nb,
+                      void* __restrict__ out, int dtype, bool wide) {
+    const uint32_t gid = blockIdx.x * 256u + threadIdx.x, r = gid >> l2;
+    if (r >= n) return;
+    for (int piece = (int)(gid & ((1u << l2) - 1)); piece < np; piece += 1 << l2) {
+        const size_t blk = (size_t)r * nb + (piece >> 2);
+        const uint8_t* s = codes + blk * 16 + (piece & 3) * 4;
+        const uint32_t w = wide ? *(const uint32_t*)s : s[0] | (uint32_t)s[1] << 8 | (uint32_t)s[2] << 16 | (uint32_t)s[3] << 24;
+        float v[8];
+        mx_decode8(w, scales[blk], v);
+        store8(out, dtype, (size_t)r * d + piece * 8, v, d - piece * 8, wide);
+    }
 }
 
 // max |x|^2 over rows [row0, row0 + n) of an mx4 index, for the margin rule (rescore_kernel), as float bits. A row with a
@@ -213,15 +217,15 @@ mx4_norm_max_kernel(const uint8_t* __restrict__ X, const uint8_t* __restrict__ X
         const int64_t row = g * 32 + l31;
         float acc = 0.f;
         for (int ks = 0; ks < nks; ++ks) {
-            const uint4 c = *(const uint4*)(X + ((size_t)g * nks + ks) * MX_SET_BYTES + l31 * 32 + h * 16);
-            const float sc = mx_scale_f32(Xs[mx_scale_at(row, 2 * ks + h, nkq)]);
+            const uint4 c = *(const uint4*)(X + mx_code_at(row, 2 * ks + h, nks));
+            const uint32_t byte = Xs[mx_scale_at(row, 2 * ks + h, nkq)];
             const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float v[8];
-                mx_decode8(w[i], v);
+                mx_decode8(w[i], byte, v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { const float y = v[e] * sc; acc = fmaf(y, y, acc); }
+                for (int e = 0; e < 8; ++e) acc = fmaf(v[e], v[e], acc);
             }
         }
         acc += __shfl_xor(acc, 32);
@@ -233,52 +237,50 @@ mx4_norm_max_kernel(const uint8_t* __restrict__ X, const uint8_t* __restrict__ X
 }
 
 // ---- lookup ----------------------------------------------------------------------------------------------------
-// out[i] = scale[i] * row(ids[i]) for an index of any storage (xfmt 0: fp32 tiles of 128 rows, 1: bf16 tiles of 256, 2:
-// mx4). One thread per eight elements of an output row. The product is rounded to fp32, then once to the output type.
-// The empty slot id -1 gives a row of zeros; so does any other id outside the index, which also sets *err.
+// out[i] = scale[i] * row(ids[i]) for an index of any storage (XFMT 0: fp32 tiles of 128 rows, 1: bf16 tiles of 256, 2: mx4).
+// The product is rounded to fp32, then once to the output type. The empty slot id -1 gives a row of zeros; so does any other
+// id outside the index, which also sets *err.
+template <int XFMT>
 __global__ void __launch_bounds__(256)
-lookup_kernel(const void* __restrict__ X, const uint8_t* __restrict__ Xs, int xfmt, int nks, int nkq, int64_t id_base, int64_t N,
-              const int64_t* __restrict__ ids, const float* __restrict__ scale, uint32_t total, uint64_t magic, int np, int d,
+lookup_kernel(const void* __restrict__ X, const uint8_t* __restrict__ Xs, int nks, int nkq, int64_t id_base, int64_t N,
+              const int64_t* __restrict__ ids, const float* __restrict__ scale, uint32_t n, int l2, int np, int d,
               void* __restrict__ out, int dtype, bool wide, int* err) {
-    const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
-    if (gid >= total) return;
-    const uint32_t i = np == 1 ? gid : div_by(gid, magic);
-    const int piece = (int)(gid - i * (uint32_t)np);
+    const uint32_t gid = blockIdx.x * 256u + threadIdx.x, i = gid >> l2;
+    if (i >= n) return;
     const int64_t id = ids[i];
     const uint64_t row = (uint64_t)id - (uint64_t)id_base;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (row < (uint64_t)N) {
-        const float s = scale ? scale[i] : 1.f;
-        if (xfmt == 2) {
-            const int b = piece >> 2;
-            const uint32_t w = *(const uint32_t*)((const uint8_t*)X + mx_code_at((int64_t)row, b, nks) + (piece & 3) * 4);
-            const float sc = mx_scale_f32(Xs[mx_scale_at((int64_t)row, b, nkq)]);
-            mx_decode8(w, v);
+    const float s = scale ? scale[i] : 1.f;
+    const bool have = row < (uint64_t)N;
+    const int first = (int)(gid & ((1u << l2) - 1));
+    if (!have && id != -1 && first == 0) *err = 1;
+    for (int piece = first; piece < np; piece += 1 << l2) {
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (have) {
+            if constexpr (XFMT == 2) {
+                const int b = piece >> 2;
+                const uint32_t w = *(const uint32_t*)((const uint8_t*)X + mx_code_at((int64_t)row, b, nks) + (piece & 3) * 4);
+                mx_decode8(w, Xs[mx_scale_at((int64_t)row, b, nkq)], v);
+            } else if constexpr (XFMT == 1) {
+                const int64_t tile = (int64_t)row / HBD;
+                const int rr = (int)(row - (uint64_t)tile * HBD), c = (piece & 3) ^ ((rr >> 2) & 3);
+                const uint4 w = *(const uint4*)((const char*)X + (((size_t)tile * nks + (piece >> 2)) * HBD + rr) * 64 + c * 16);
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= sc;
-        } else if (xfmt == 1) {
-            const int64_t tile = (int64_t)row / HBD;
-            const int rr = (int)(row - (uint64_t)tile * HBD), c = (piece & 3) ^ ((rr >> 2) & 3);
-            const uint4 w = *(const uint4*)((const char*)X + (((size_t)tile * nks + (piece >> 2)) * HBD + rr) * 64 + c * 16);
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                for (int e = 0; e < 4; ++e) { v[2 * e] = bf16_lo(ws[e]); v[2 * e + 1] = bf16_hi(ws[e]); }
+            } else {
+                const int64_t tile = (int64_t)row / BD;
+                const int rr = (int)(row - (uint64_t)tile * BD), sw = (rr >> 2) & 3, c0 = (piece & 1) * 2;
+                const char* line = (const char*)X + (((size_t)tile * nks + (piece >> 1)) * BD + rr) * 64;
+                const f32x4 a = *(const f32x4*)(line + (c0 ^ sw) * 16), b = *(const f32x4*)(line + ((c0 + 1) ^ sw) * 16);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { v[2 * e] = bf16_lo(ws[e]); v[2 * e + 1] = bf16_hi(ws[e]); }
-        } else {
-            const int64_t tile = (int64_t)row / BD;
-            const int rr = (int)(row - (uint64_t)tile * BD), sw = (rr >> 2) & 3, c0 = (piece & 1) * 2;
-            const char* line = (const char*)X + (((size_t)tile * nks + (piece >> 1)) * BD + rr) * 64;
-            const f32x4 a = *(const f32x4*)(line + (c0 ^ sw) * 16), b = *(const f32x4*)(line + ((c0 + 1) ^ sw) * 16);
+                for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+            }
+            if (scale)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+                for (int e = 0; e < 8; ++e) v[e] *= s;
         }
-        if (scale)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= s;
-    } else if (id != -1 && piece == 0) {
-        *err = 1;
+        store8(out, dtype, (size_t)i * d + piece * 8, v, d - piece * 8, wide);
     }
-    const int left = d - piece * 8;
-    store8(out, dtype, (size_t)i * d + piece * 8, v, left < 8 ? left : 8, wide);
 }
 
 // ---- queries for the matrix core -------------------------------------------------------------------------------
@@ -402,18 +404,17 @@ struct MxParams {
     int64_t N;                   // rows of the index
     int nq, d, nks, nkq;
     int S;                       // splits: workgroups that share a query block
-    int qc;                      // quads of the query block that LDS holds at a time (nkq: all, staged once)
-    int64_t g0, gstep;           // wave tile t covers groups g0 + t * gstep, + 1
+    int64_t g0, gstep;           // wave tile t covers the MX_RG groups from g0 + t * gstep
     int64_t ntiles;
     // scores
     float* out;                  // [nq][ld]
-    int64_t ld, row0, n;         // columns 0 .. n - 1 are rows row0 ..; row0 < 0: column = 64 t + row of the tile
+    int64_t ld, row0, n;         // columns 0 .. n - 1 are rows row0 ..; row0 < 0: column = MX_TILE t + row of the tile
     const void* q;               // the caller's queries (recomputation of those with NaN / inf elements), or null
     int q_dtype;
     const MxQueryInfo* info;
     // search
     const float* tau;            // [nq] floor: a hit scores above it, or equals it with row < row_below
-    const int64_t* row_below;    // [nq]
+    const uint32_t* row_below;   // [nq] a multiple of 32
     uint64_t* cand;              // [nq][S][cap] keys of the hits
     int* cnt;                    // [nq][S]
     int* todo;                   // [nq] set to 1 when a list overflows
@@ -436,17 +437,31 @@ __device__ __forceinline__ float mx4_plain_dot(const MxParams& p, int q, int64_t
 
 enum { MX_SCORES = 0, MX_SEARCH = 1 };
 
-// One wave: 64 rows (two groups) x BQ = 32 CG queries; 8 waves a workgroup, which share the query block in LDS and nothing
-// else: while the whole block fits (qc == nkq) the main loop has no barrier. A quad of K-sets (256 elements) is the step of
-// the loop: its row operands were fetched one step earlier (across tiles too), and per K-set, part and pair of 32 x 32
-// blocks one MFMA runs. Tiles are dealt round-robin over the waves of a query block's S workgroups.
-// When the query block does not fit, its quads go through LDS qc at a time, all waves in step.
-template <int CG, int PARTS, int FMT, int MODE>
+template <int I, int N, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<I + 1, N>(f);
+    }
+}
+
+// One wave: 128 rows (RG = 4 groups) x BQ = 32 CG queries; 8 waves a workgroup, which share the query block in LDS and
+// nothing else: while the whole block fits (RESIDENT) the main loop has no barrier. The loop steps through quads of K-sets
+// (256 elements), the quads of a tile and on to the next tile. A K-set's row operands wait in registers: the slot of a
+// K-set is loaded again, for the next quad, as soon as its last MFMA is issued, so four K-sets are in flight (16 KiB a wave,
+// 128 KiB a CU). The query operands of the next part are read from LDS while the current part is multiplied: RG x CG MFMAs
+// per CG reads of 24 bytes a lane.
+// Tiles are dealt round-robin over a query block's S workgroups, then over their waves. When the query block does not fit (long
+// vectors), its quads go through LDS one at a time, all waves in step.
+// MX_SCORES: queries are the A operand, so that a lane holds one row and a store instruction writes two lines of 32
+// consecutive columns (with rows as A: 32 pieces of 32 bytes, one query each; 8192 x 32768 scores took 500 us so).
+// MX_SEARCH: rows are the A operand: a lane holds 16 rows of one query and its floor.
+template <int CG, int PARTS, int FMT, int MODE, bool RESIDENT>
 __global__ void __launch_bounds__(MX_THREADS)
 mx4_product_kernel(const MxParams p) {
-    constexpr int BQ = 32 * CG, PART = mx_part_bytes<FMT>(BQ), QUAD = PARTS * PART;
+    constexpr int RG = MX_RG, BQ = 32 * CG, PART = mx_part_bytes<FMT>(BQ), QUAD = PARTS * PART, CODES = mx_code_bytes<FMT>();
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int* cnts = (int*)(smem + (size_t)p.qc * QUAD);                    // [BQ]  (MX_SEARCH)
+    int* cnts = (int*)(smem + (size_t)(RESIDENT ? p.nkq : 1) * QUAD);   // [BQ]  (MX_SEARCH)
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nqb = (int)gridDim.x / p.S;
@@ -457,7 +472,8 @@ mx4_product_kernel(const MxParams p) {
     const char* qblock = (const char*)p.Q + (size_t)qb * p.nkq * QUAD;
 
     float tau[CG];
-    int64_t below[CG];
+    uint32_t below[CG];
+    int redo = 0;                       // MX_SCORES: a query of this block is not finite
     if constexpr (MODE == MX_SEARCH) {
 #pragma unroll
         for (int c = 0; c < CG; ++c) {
@@ -466,183 +482,220 @@ mx4_product_kernel(const MxParams p) {
             below[c] = q < p.nq ? p.row_below[q] : 0;
         }
         for (int i = tid; i < BQ; i += MX_THREADS) cnts[i] = 0;
-    }
-    int redo = 0;                                                       // MX_SCORES: this lane's queries that are not finite
-    if constexpr (MODE == MX_SCORES) {
-        if (p.q)
+    } else if (p.q) {
 #pragma unroll
-            for (int c = 0; c < CG; ++c) {
-                const int q = qb * BQ + c * 32 + l31;
-                if (q < p.nq && !(p.info[q].sumsq <= FLT_MAX)) redo |= 1 << c;
-            }
+        for (int c = 0; c < CG; ++c) {
+            const int q = qb * BQ + c * 32 + l31;
+            redo |= q < p.nq && !(p.info[q].sumsq <= FLT_MAX) ? 1 : 0;
+        }
     }
-    auto stage = [&](int quad0) {
-        const int n16 = (p.nkq - quad0 < p.qc ? p.nkq - quad0 : p.qc) * (QUAD / 16);
+    auto stage = [&](int quad0, int quads) {
         const uint4* s = (const uint4*)(qblock + (size_t)quad0 * QUAD);
-        for (int i = tid; i < n16; i += MX_THREADS) ((uint4*)smem)[i] = s[i];
+#pragma unroll 4
+        for (int i = tid; i < quads * (QUAD / 16); i += MX_THREADS) ((uint4*)smem)[i] = s[i];
     };
-    const bool resident = p.qc >= p.nkq;
-    if (resident) stage(0);
+    if constexpr (RESIDENT) stage(0, p.nkq);
     __syncthreads();
 
     const int64_t per_round = (int64_t)p.S * 8;
     const int64_t rounds = (p.ntiles + per_round - 1) / per_round;
-    const int64_t tile0 = (int64_t)split * 8 + wave;
+    const int64_t tile0 = (int64_t)wave * p.S + split;
     const size_t group_bytes = (size_t)p.nks * MX_SET_BYTES, group_scales = (size_t)p.nkq * 256;
+    const uint32_t lane_pair = l31 * 64 + h * 16, lane_alone = l31 * 32 + h * 16, lane_scale = (uint32_t)l31 * p.nkq * 8 + h * 4;
 
-    struct Operands { uint4 a[4][MX_RG]; uint32_t s[MX_RG]; };
-    Operands A0, A1;
-    auto fetch = [&](Operands& o, int64_t tile, int quad) {
-        if (tile >= p.ntiles) return;
-        const int64_t g = p.g0 + tile * p.gstep;
+    // ---- row operands
+    uint4 A[4][RG];
+    uint32_t xs[RG], xs_next[RG];
+    auto group_of = [&](int64_t tile) { return p.g0 + (tile < p.ntiles ? tile : p.ntiles - 1) * p.gstep; };
+    // (buffer loads: the tile's address in scalar registers, the lane's part a 32-bit offset)
+    const int set_bytes = (int)group_bytes, scale_bytes = (int)group_scales;
+    auto load_slot = [&](uint4 (&a)[RG], const __amdgpu_buffer_rsrc_t x, int ks) {
+        ks = ks < p.nks ? ks : p.nks - 1;                              // (behind the last K-set: loaded, not multiplied)
+        const bool alone = (ks & 1) == 0 && ks + 1 == p.nks;
+        const int at = (ks >> 1) * 2 * MX_SET_BYTES + (ks & 1) * 32;
 #pragma unroll
-        for (int r = 0; r < MX_RG; ++r) {
-            const uint8_t* x = p.X + (size_t)(g + r) * group_bytes + (size_t)quad * 4 * MX_SET_BYTES + l31 * 32 + h * 16;
-            o.s[r] = *(const uint32_t*)(p.Xs + (size_t)(g + r) * group_scales + (size_t)l31 * p.nkq * 8 + quad * 8 + h * 4);
+        for (int r = 0; r < RG; ++r)
+            a[r] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(x, alone ? lane_alone : lane_pair, at + r * set_bytes, 0));
+    };
+    auto load_scales = [&](uint32_t (&s)[RG], const __amdgpu_buffer_rsrc_t x, int quad) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (quad * 4 + j < p.nks) o.a[j][r] = *(const uint4*)(x + j * MX_SET_BYTES);
-        }
+        for (int r = 0; r < RG; ++r) s[r] = __builtin_amdgcn_raw_buffer_load_b32(x, lane_scale, quad * 8 + r * scale_bytes, 0);
+    };
+    constexpr int RAW = 0x00027000;                                    // a raw buffer of 32-bit data
+    auto codes_of = [&](int64_t g) { return __builtin_amdgcn_make_buffer_rsrc((void*)(p.X + (size_t)g * group_bytes), 0, RG * set_bytes, RAW); };
+    auto scales_of = [&](int64_t g) { return __builtin_amdgcn_make_buffer_rsrc((void*)(p.Xs + (size_t)g * group_scales), 0, RG * scale_bytes, RAW); };
+
+    // ---- query operands: 32 queries of one part and K-set at a time
+    struct Part { uint4 lo; uint2 hi; };
+    Part B[2];
+    uint32_t qs[PARTS][CG], qs_first[CG];
+    const uint32_t q16 = (h * BQ + l31) * 16, q8 = (h * BQ + l31) * 8, q4 = (h * BQ + l31) * 4;
+    auto load_part = [&](Part& b, const char* quad_lds, int j, int part, int c) {
+        const char* at = quad_lds + part * PART;
+        b.lo = *(const uint4*)(at + q16 + (j * 2 * BQ + c * 32) * 16);
+        if constexpr (FMT == MX_E2M3) b.hi = *(const uint2*)(at + q8 + BQ * 128 + (j * 2 * BQ + c * 32) * 8);
+    };
+    auto load_part_scales = [&](uint32_t (&s)[CG], const char* quad_lds, int part) {
+#pragma unroll
+        for (int c = 0; c < CG; ++c) s[c] = *(const uint32_t*)(quad_lds + part * PART + BQ * 8 * CODES + q4 + c * 128);
     };
 
-    f32x16 acc[MX_RG][CG];
+    f32x16 acc[RG][CG];
     auto clear = [&]() {
 #pragma unroll
-        for (int r = 0; r < MX_RG; ++r)
+        for (int r = 0; r < RG; ++r)
 #pragma unroll
             for (int c = 0; c < CG; ++c)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[r][c][i] = 0.f;
     };
-    clear();
 
-    auto multiply = [&](const Operands& o, int quad) {
-        const char* qq = smem + (size_t)(quad % p.qc) * QUAD;
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-            uint32_t qs[CG];
-#pragma unroll
-            for (int c = 0; c < CG; ++c)
-                qs[c] = *(const uint32_t*)(qq + part * PART + BQ * 8 * mx_code_bytes<FMT>() + (h * BQ + c * 32 + l31) * 4);
-            auto kset = [&](auto jc) {
-                constexpr int j = decltype(jc)::value;
-                if (quad * 4 + j >= p.nks) return;
-#pragma unroll
-                for (int c = 0; c < CG; ++c) {
-                    const char* at = qq + part * PART + ((j * 2 + h) * BQ + c * 32 + l31) * 16;
-                    const uint4 lo = *(const uint4*)at;
-                    i32x8 b = {(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, 0, 0, 0, 0};
-                    if constexpr (FMT == MX_E2M3) {
-                        const uint2 hi = *(const uint2*)(qq + part * PART + BQ * 128 + ((j * 2 + h) * BQ + c * 32 + l31) * 8);
-                        b[4] = (int)hi.x;
-                        b[5] = (int)hi.y;
-                    }
-#pragma unroll
-                    for (int r = 0; r < MX_RG; ++r) {
-                        const i32x8 a = {(int)o.a[j][r].x, (int)o.a[j][r].y, (int)o.a[j][r].z, (int)o.a[j][r].w, 0, 0, 0, 0};
-                        acc[r][c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc[r][c], MX_E2M1, FMT, j, (int)o.s[r], j, (int)qs[c]);
-                    }
-                }
-            };
-            kset(std::integral_constant<int, 0>{});
-            kset(std::integral_constant<int, 1>{});
-            kset(std::integral_constant<int, 2>{});
-            kset(std::integral_constant<int, 3>{});
-        }
-    };
-
-    // column of the lane's first row in group r of a tile (MX_SCORES)
-    auto column = [&](int64_t tile, int r) {
-        return (p.row0 < 0 ? tile * MX_TILE + r * 32 : (p.g0 + tile * p.gstep + r) * 32 - p.row0) + 4 * h;
-    };
     auto finish = [&](int64_t tile) {
         const int64_t g = p.g0 + tile * p.gstep;
+        if constexpr (MODE == MX_SCORES) {
 #pragma unroll
-        for (int c = 0; c < CG; ++c) {
-            const int ql = c * 32 + l31, q = qb * BQ + ql;
-            if constexpr (MODE == MX_SCORES) {
-                if (q >= p.nq) continue;
+            for (int r = 0; r < RG; ++r) {
+                const int64_t col = (p.row0 < 0 ? tile * MX_TILE + r * 32 : (g + r) * 32 - p.row0) + l31;
+                if (col < 0 || col >= p.n) continue;
 #pragma unroll
-                for (int r = 0; r < MX_RG; ++r) {
-                    const int64_t col0 = column(tile, r);
-                    float* o = p.out + (size_t)q * p.ld;
+                for (int c = 0; c < CG; ++c) {
+                    const int q0 = qb * BQ + c * 32 + 4 * h;
+                    float* o = p.out + (size_t)q0 * p.ld + col;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int64_t col = col0 + 8 * i;
-                        const f32x4 v = {acc[r][c][4 * i], acc[r][c][4 * i + 1], acc[r][c][4 * i + 2], acc[r][c][4 * i + 3]};
-                        if (col >= 0 && col + 4 <= p.n) {
-                            __builtin_memcpy(o + col, &v, 16);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (col + e >= 0 && col + e < p.n) o[col + e] = v[e];
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        const int at = (i & 3) + 8 * (i >> 2);
+                        if (q0 + at < p.nq) o[(size_t)at * p.ld] = acc[r][c][i];
                     }
                 }
-            } else {
-#pragma unroll
-                for (int r = 0; r < MX_RG; ++r) {
-                    float g4[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        g4[i] = fmaxf(fmaxf(acc[r][c][4 * i], acc[r][c][4 * i + 1]), fmaxf(acc[r][c][4 * i + 2], acc[r][c][4 * i + 3]));
-                    if (!__any(fmaxf(fmaxf(g4[0], g4[1]), fmaxf(g4[2], g4[3])) >= tau[c])) continue;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (!__any(g4[i] >= tau[c])) continue;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float sc = acc[r][c][4 * i + e];
-                            const int64_t doc = (g + r) * 32 + 4 * h + 8 * i + e;
-                            if ((sc > tau[c] || (sc == tau[c] && doc < below[c])) && doc < p.N) {
-                                const int pos = atomicAdd(&cnts[ql], 1);
-                                if (pos < p.cap) p.cand[((size_t)q * p.S + split) * p.cap + pos] = make_key(sc, (uint32_t)doc);
-                            }
-                        }
+                if (redo)
+#pragma unroll 1
+                    for (int i = 0; i < BQ; ++i) {
+                        const int q = qb * BQ + i;
+                        if (((i >> 2) & 1) == h && q < p.nq && !(p.info[q].sumsq <= FLT_MAX))
+                            p.out[(size_t)q * p.ld + col] = mx4_plain_dot(p, q, (g + r) * 32 + l31);
                     }
+            }
+        } else {
+            // Hits of a lane: 16 rows of one query in each of the RG groups, as a bit mask per group; then one LDS atomic
+            // per lane and 32 queries takes room for all of them (an atomic per hit, each waited for, cost more than the
+            // products at 1000 hits of 500k rows). row_below is a multiple of 32: a group lies on one side of it.
+#pragma unroll
+            for (int c = 0; c < CG; ++c) {
+                uint32_t mask[RG];
+                int n = 0;
+#pragma unroll
+                for (int r = 0; r < RG; ++r) {
+                    const uint32_t doc0 = (uint32_t)(g + r) * 32;
+                    float m = acc[r][c][0];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) m = fmaxf(m, acc[r][c][i]);
+                    const float floor = doc0 < below[c] ? f32_below(tau[c]) : tau[c];      // hits score above it
+                    mask[r] = 0;
+                    if (__any(m > floor)) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) mask[r] |= acc[r][c][i] > floor ? 1u << i : 0u;
+                        if (doc0 + 32 > (uint32_t)p.N)                                     // rows behind the last one
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if (doc0 + 4 * h + (i & 3) + 8 * (i >> 2) >= (uint32_t)p.N) mask[r] &= ~(1u << i);
+                        n += __popc(mask[r]);
+                    }
+                }
+                if (!__any(n)) continue;
+                // (the empty asm keeps the compiler from holding these in registers through the main loop)
+                uint32_t ql = c * 32 + l31, h4 = 4 * h;
+                asm volatile("" : "+v"(ql), "+v"(h4));
+                int pos = n ? atomicAdd(&cnts[ql], n) : 0;
+                uint64_t* list = p.cand + ((size_t)(qb * BQ + ql) * p.S + split) * p.cap;
+#pragma unroll
+                for (int r = 0; r < RG; ++r) {
+                    if (!__any(mask[r])) continue;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (mask[r] >> i & 1) {
+                            if (pos < p.cap) list[pos] = make_key(acc[r][c][i], (uint32_t)(g + r) * 32 + h4 + (i & 3) + 8 * (i >> 2));
+                            ++pos;
+                        }
                 }
             }
         }
-        if constexpr (MODE == MX_SCORES)
-            if (__any(redo != 0)) {
-#pragma unroll 1
-                for (int i = 0; i < CG * MX_RG * 16; ++i) {
-                    const int c = i / (MX_RG * 16), r = (i >> 4) % MX_RG, at = (i & 3) + 8 * ((i >> 2) & 3);
-                    const int64_t col = column(tile, r) + at;
-                    const int q = qb * BQ + c * 32 + l31;
-                    if ((redo >> c & 1) && col >= 0 && col < p.n) p.out[(size_t)q * p.ld + col] = mx4_plain_dot(p, q, (g + r) * 32 + 4 * h + at);
-                }
-            }
     };
 
-    // the flattened sequence of (round, quad) steps
-    int64_t round = 0;
-    int quad = 0;
-    fetch(A0, tile0, 0);
-    auto step = [&](Operands& cur, Operands& nxt) -> bool {            // false: that was the last one
-        const int64_t tile = tile0 + round * per_round;
-        if (!resident && quad % p.qc == 0) {
-            __syncthreads();
-            stage(quad);
-            __syncthreads();
+    if (!RESIDENT || tile0 < p.ntiles) {
+        redo = __any(redo);
+        int64_t tile = tile0, round = 0;
+        int quad = 0;
+        {
+            const int64_t g = group_of(tile);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) load_slot(A[j], codes_of(g), j);
+            load_scales(xs, scales_of(g), 0);
         }
-        const bool last = quad + 1 == p.nkq;
-        const int64_t nround = last ? round + 1 : round;
-        const int nquad = last ? 0 : quad + 1;
-        if (nround < rounds) fetch(nxt, tile0 + nround * per_round, nquad);
-        if (tile < p.ntiles) {
-            multiply(cur, quad);
-            if (last) {
-                finish(tile);
-                clear();
+        if constexpr (RESIDENT) {
+            load_part(B[0], smem, 0, 0, 0);
+            load_part_scales(qs_first, smem, 0);
+        }
+        clear();
+        while (true) {
+            const bool last = quad + 1 == p.nkq;
+            const int nquad = last ? 0 : quad + 1;
+            const int64_t ntile = last ? tile + per_round : tile;
+            const int64_t ng = group_of(ntile);
+            const char* here = smem + (RESIDENT ? (size_t)quad * QUAD : 0);
+            const char* there = smem + (RESIDENT ? (size_t)nquad * QUAD : 0);
+            if constexpr (!RESIDENT) {
+                __syncthreads();
+                stage(quad, 1);
+                __syncthreads();
+                load_part(B[0], here, 0, 0, 0);
+                load_part_scales(qs_first, here, 0);
             }
+            const __amdgpu_buffer_rsrc_t next = codes_of(ng);
+            load_scales(xs_next, scales_of(ng), nquad);
+#pragma unroll
+            for (int c = 0; c < CG; ++c) qs[0][c] = qs_first[c];
+            static_for<0, 4 * PARTS * CG>([&](auto tc) {
+                constexpr int T = decltype(tc)::value, j = T / (PARTS * CG), part = T / CG % PARTS, c = T % CG;
+                constexpr int U = T + 1, jn = U / (PARTS * CG), pn = U / CG % PARTS, cn = U % CG;
+                const Part& b = B[T & 1];
+                Part& bn = B[U & 1];
+                if constexpr (jn < 4) {
+                    load_part(bn, here, jn, pn, cn);
+                    if constexpr (jn == 0 && cn == 0) load_part_scales(qs[pn], here, pn);
+                } else if constexpr (RESIDENT) {
+                    load_part(bn, there, 0, 0, 0);
+                    load_part_scales(qs_first, there, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (quad * 4 + j < p.nks) {
+                    i32x8 qv = {(int)b.lo.x, (int)b.lo.y, (int)b.lo.z, (int)b.lo.w, 0, 0, 0, 0};
+                    if constexpr (FMT == MX_E2M3) {
+                        qv[4] = (int)b.hi.x;
+                        qv[5] = (int)b.hi.y;
+                    }
+#pragma unroll
+                    for (int r = 0; r < RG; ++r) {
+                        const i32x8 xv = {(int)A[j][r].x, (int)A[j][r].y, (int)A[j][r].z, (int)A[j][r].w, 0, 0, 0, 0};
+                        if constexpr (MODE == MX_SCORES)
+                            acc[r][c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qv, xv, acc[r][c], FMT, MX_E2M1, j, (int)qs[part][c], j, (int)xs[r]);
+                        else
+                            acc[r][c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xv, qv, acc[r][c], MX_E2M1, FMT, j, (int)xs[r], j, (int)qs[part][c]);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (part == PARTS - 1 && c == CG - 1) load_slot(A[j], next, nquad * 4 + j);
+            });
+#pragma unroll
+            for (int r = 0; r < RG; ++r) xs[r] = xs_next[r];
+            if (last) {
+                if (tile < p.ntiles) finish(tile);
+                clear();
+                if (++round == rounds || (RESIDENT && ntile >= p.ntiles)) break;
+            }
+            tile = ntile;
+            quad = nquad;
         }
-        round = nround;
-        quad = nquad;
-        return round < rounds;
-    };
-    if (rounds > 0)
-        while (step(A0, A1) && step(A1, A0)) {}
+    }
 
     if constexpr (MODE == MX_SEARCH) {
         __syncthreads();
@@ -657,25 +710,73 @@ mx4_product_kernel(const MxParams p) {
 }
 
 // ---- the floor of a search -------------------------------------------------------------------------------------
-// A search scores a sample of the index first (MX_SAMPLE rows, whole tiles at equal distances) and takes its j-th best
-// score as the floor every hit has to reach: with j well above the share of the wanted list that falls into the sample,
-// about j / sample of the index passes (the host chooses j: mx4_floor_rank), which is a few times the list. Equal scores
-// are ordered by row as everywhere: where the j-th best sits among equals, rows up to its share of the index pass.
-// One workgroup of 1024 per query: radix selection, 8 bits a pass, on the scores held in registers.
+// A search scores a sample of the index first (whole tiles at equal distances) and takes about its j-th best score as the
+// floor every hit has to reach: with j well above the share of the wanted list that falls into the sample, about j / sample
+// of the index passes (the host chooses j: mx4_pass), which is a small multiple of the list.
+// One workgroup of 1024 per query, the sample's scores in registers. A histogram of 2047 steps of 2^-10 of a binade below
+// the best score finds the step that the j-th lies in, and its lower edge is the floor. Where it lies lower, or in a step
+// with far more than j scores (equal scores), the j-th is found exactly by radix selection, and scores equal to it pass up
+// to a row: its share of the index, as equal scores are ordered by row.
+template <int PER>
 __global__ void __launch_bounds__(1024)
-mx4_floor_kernel(const float* __restrict__ sample, int m, int j, int64_t N, float* __restrict__ tau, int64_t* __restrict__ row_below) {
-    constexpr int PER = MX_SAMPLE / 1024;
-    __shared__ int hist[256];
+mx4_floor_kernel(const float* __restrict__ sample, int j, int64_t N, float* __restrict__ tau, uint32_t* __restrict__ row_below) {
+    constexpr int M = PER * 1024;
+    __shared__ int hist[2048];
+    __shared__ uint32_t s_wave[16];
     __shared__ uint32_t s_prefix;
-    __shared__ int s_need, s_wave[16];
+    __shared__ int s_need, s_bin;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t q = blockIdx.x;
-    uint32_t v[PER];                                           // entries tid * PER .. + PER - 1: a thread's are neighbours
+    // entries 4 tid .. + 3 of every 4096: ordered score bits, 0 for what is never a hit (NaN, -inf)
+    uint32_t v[PER];
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i += 4) {
+        const float4 s4 = *(const float4*)(sample + q * (int64_t)M + i * 1024 + tid * 4);
+        const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[i + e] = s[e] > -FLT_MAX ? f32_ordered(s[e]) : 0u;
+            best = max(best, v[i + e]);
+        }
+    }
+    hist[tid] = 0;
+    hist[tid + 1024] = 0;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, off));
+    if (lane == 0) s_wave[wave] = best;
+    if (tid == 0) s_bin = -1;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 16; ++w) best = max(best, s_wave[w]);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int e = tid * PER + i;
-        const float s = e < m ? sample[q * (int64_t)m + e] : -INFINITY;
-        v[i] = s > -FLT_MAX ? f32_ordered(s) : 0u;             // NaN and -inf are never hits
+        const uint32_t bin = (best - v[i]) >> 13;
+        if (v[i] && bin < 2047) atomicAdd(&hist[bin], 1);
+    }
+    __syncthreads();
+    // cumulative counts: thread t owns bins 2 t, 2 t + 1
+    const int c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
+    int run = c0 + c1;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) { const int x = __shfl_up(run, off); if (lane >= off) run += x; }
+    if (lane == 63) s_wave[wave] = (uint32_t)run;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) run += (int)s_wave[w];
+    const int before = run - c0 - c1;
+    if (before < j && run >= j) {
+        const bool second = before + c0 < j;
+        if ((second ? run : before + c0) <= 2 * j + 64) s_bin = 2 * tid + (second ? 1 : 0);
+    }
+    __syncthreads();
+    if (s_bin >= 0) {
+        if (tid == 0) {
+            const uint32_t steps = ((uint32_t)s_bin << 13) + 0x1fffu;       // the step's lowest score: this far below the best
+            const uint32_t least = f32_ordered(-FLT_MAX) + 2;
+            tau[q] = best >= least && best - least >= steps ? f32_below(f32_unordered(best - steps)) : -FLT_MAX;
+            row_below[q] = 0;
+        }
+        return;
     }
     if (tid == 0) { s_prefix = 0; s_need = j; }
     for (int shift = 24; shift >= 0; shift -= 8) {
@@ -686,30 +787,14 @@ mx4_floor_kernel(const float* __restrict__ sample, int m, int j, int64_t N, floa
         for (int i = 0; i < PER; ++i)
             if (v[i] && (shift == 24 || (v[i] >> (shift + 8)) == (prefix >> (shift + 8)))) atomicAdd(&hist[(v[i] >> shift) & 255], 1);
         __syncthreads();
-        if (wave == 0) {
-            // the bucket that holds the need-th largest: lane l owns buckets 255 - 4 l .. 252 - 4 l
-            int mine[4], sum = 0;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) { mine[u] = hist[255 - 4 * lane - u]; sum += mine[u]; }
-            int run = sum;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) { const int x = __shfl_up(run, off); if (lane >= off) run += x; }
-            const int need = s_need;
-            int before = run - sum;
-            const bool here = before < need && run >= need;
-            if (here) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if (before < need && before + mine[u] >= need) {
-                        s_prefix = prefix | (uint32_t)(255 - 4 * lane - u) << shift;
-                        s_need = need - before;
-                        before = 0x7fffffff;                   // found
-                    } else if (before != 0x7fffffff) {
-                        before += mine[u];
-                    }
-                }
+        if (tid == 0) {
+            int b = 255, acc = 0;
+            while (b >= 0 && acc + hist[b] < s_need) acc += hist[b--];
+            if (b < 0) s_need = 0;                             // fewer than j numbers in the sample: no floor
+            else {
+                s_need -= acc;
+                s_prefix = prefix | (uint32_t)b << shift;
             }
-            if (!__any(here) && lane == 0) { s_prefix = 0; s_need = 0; }      // fewer than j numbers in the sample
         }
         __syncthreads();
         if (s_need == 0) break;
@@ -720,29 +805,179 @@ mx4_floor_kernel(const float* __restrict__ sample, int m, int j, int64_t N, floa
         if (tid == 0) { tau[q] = -FLT_MAX; row_below[q] = 0; }
         return;
     }
-    int eq = 0;
+    // row order: entries i * 1024 + 4 tid + e, i a multiple of 4
+    int done = 0;
+    for (int i = 0; i < PER; i += 4) {
+        int eq = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) eq += v[i] == t ? 1 : 0;
-    int run = eq;
+        for (int k = 0; k < PER; k += 4)
+            if (k == i)
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) { const int x = __shfl_up(run, off); if (lane >= off) run += x; }
-    if (lane == 63) s_wave[wave] = run;
-    __syncthreads();
-    int before = run - eq;
-    for (int w = 0; w < wave; ++w) before += s_wave[w];
-    if (before < need && before + eq >= need) {
-        int k = before;
-        for (int i = 0; i < PER; ++i)
-            if (v[i] == t && ++k == need) {
+                for (int e = 0; e < 4; ++e) eq |= v[k + e] == t ? 1 << e : 0;
+        int at = __popc((uint32_t)eq);
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) { const int x = __shfl_up(at, off); if (lane >= off) at += x; }
+        __syncthreads();
+        if (lane == 63) s_wave[wave] = (uint32_t)at;
+        __syncthreads();
+        int total = 0;
+        for (int w = 0; w < 16; ++w) { if (w < wave) at += (int)s_wave[w]; total += (int)s_wave[w]; }
+        int k = done + at - __popc((uint32_t)eq);              // equals before this thread's
+        for (int e = 0; e < 4; ++e)
+            if ((eq >> e & 1) && ++k == need) {
                 tau[q] = f32_unordered(t);
-                row_below[q] = ((int64_t)(tid * PER + i + 1) * N + m - 1) / m;
+                const int64_t rows = ((int64_t)(i * 1024 + tid * 4 + e + 1) * N + M - 1) / M;
+                row_below[q] = (uint32_t)((rows + 31) / 32 * 32);
             }
+        done += total;
+        if (done >= need) return;
+    }
+}
+
+// ---- the hits of one query -> its best kc, sorted --------------------------------------------------------------
+// lists: [nq][S][cap] keys in any order, cnt[q * S + s] of them. One workgroup of 1024 per query. Few more hits than wanted
+// is the rule (mx4_floor_kernel): a histogram of the scores between the lowest and the best hit, linear in the bits, finds
+// the step that holds the kc-th; everything from that step up (a few more than kc) is sorted in LDS (Pmax slots). Should
+// that be more than the slots (equal scores), the kc-th key is found exactly, 8 bits a pass.
+constexpr int MX_HELD = 4096;            // hits that are kept in LDS between the passes
+__global__ void __launch_bounds__(1024)
+mx4_select_kernel(const uint64_t* __restrict__ lists, const int* __restrict__ cnt, int S, int cap, int kc, int Pmax, int64_t id_base,
+                  float* __restrict__ outD, int64_t* __restrict__ outI) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    uint64_t* sorted = (uint64_t*)smem;                        // [Pmax]
+    uint64_t* held = sorted + Pmax;                            // [MX_HELD]
+    int* off = (int*)(held + MX_HELD);                         // [S]
+    __shared__ int hist[2048];
+    __shared__ uint32_t s_lo[16], s_hi[16];
+    __shared__ int s_sum[16], s_total, s_bin, s_n, s_need;
+    __shared__ uint64_t s_prefix;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t q = blockIdx.x;
+    const uint64_t* base = lists + (size_t)q * S * cap;
+    // the lists' places in `held`: S <= 1024
+    const int mine = tid < S ? cnt[q * S + tid] : 0;
+    int run = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(run, o); if (lane >= o) run += x; }
+    if (lane == 63) s_sum[wave] = run;
+    hist[tid] = 0;
+    hist[tid + 1024] = 0;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) run += s_sum[w];
+    if (tid < S) off[tid] = run - mine;
+    if (tid == 1023) s_total = run;
+    if (tid == 0) { s_bin = 0; s_n = 0; }
+    __syncthreads();
+    const int T = s_total;
+    const bool keep = T <= MX_HELD;
+    // 2^g lanes to a list
+    int g = 0;
+    while ((S << (g + 1)) <= 1024) ++g;
+    auto each_key = [&](auto&& f) {
+        for (int s = tid >> g; s < S; s += 1024 >> g) {
+            const int n = (s + 1 < S ? off[s + 1] : T) - off[s];
+            for (int e = tid & ((1 << g) - 1); e < n; e += 1 << g) f(base[(size_t)s * cap + e], off[s] + e);
+        }
+    };
+    auto each_held = [&](auto&& f) {
+        if (keep) for (int e = tid; e < T; e += 1024) f(held[e]);
+        else each_key([&](uint64_t key, int) { f(key); });
+    };
+    uint32_t lo = 0xffffffffu, hi = 0;
+    each_key([&](uint64_t key, int at) {
+        const uint32_t v = (uint32_t)(key >> 32);
+        lo = min(lo, v);
+        hi = max(hi, v);
+        if (keep) held[at] = key;
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        lo = min(lo, (uint32_t)__shfl_xor((int)lo, o));
+        hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
+    }
+    if (lane == 0) { s_lo[wave] = lo; s_hi[wave] = hi; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 16; ++w) { lo = min(lo, s_lo[w]); hi = max(hi, s_hi[w]); }
+    int shift = 0;
+    if (T > kc) {
+        while (((hi - lo) >> shift) >= 2048) ++shift;
+        each_held([&](uint64_t key) { atomicAdd(&hist[(hi - (uint32_t)(key >> 32)) >> shift], 1); });
+        __syncthreads();
+        const int c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
+        int acc = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(acc, o); if (lane >= o) acc += x; }
+        if (lane == 63) s_sum[wave] = acc;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) acc += s_sum[w];
+        const int before = acc - c0 - c1;
+        if (before < kc && acc >= kc) {
+            const bool second = before + c0 < kc;
+            s_bin = 2 * tid + (second ? 1 : 0);
+            s_n = second ? acc : before + c0;
+        }
+        __syncthreads();
+    }
+    const bool few = T <= kc || s_n <= Pmax;
+    const uint32_t bin = (uint32_t)s_bin;
+    __syncthreads();
+    int m;
+    if (few) {
+        if (tid == 0) s_n = 0;
+        __syncthreads();
+        each_held([&](uint64_t key) {
+            if (T <= kc || (hi - (uint32_t)(key >> 32)) >> shift <= bin) sorted[atomicAdd(&s_n, 1)] = key;
+        });
+        __syncthreads();
+        m = s_n;
+    } else {
+        if (tid == 0) { s_prefix = 0; s_need = kc; s_n = 0; }
+        for (int sh = 56; sh >= 0; sh -= 8) {
+            if (tid < 256) hist[tid] = 0;
+            __syncthreads();
+            const uint64_t prefix = s_prefix;
+            each_held([&](uint64_t key) {
+                if (sh == 56 || (key >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[(int)(key >> sh) & 255], 1);
+            });
+            __syncthreads();
+            if (tid == 0) {
+                int b = 255, acc = 0;
+                while (b > 0 && acc + hist[b] < s_need) acc += hist[b--];
+                s_need -= acc;
+                s_prefix = prefix | (uint64_t)b << sh;
+            }
+            __syncthreads();
+        }
+        const uint64_t kth = s_prefix;                         // keys are distinct: kc of them reach it
+        each_held([&](uint64_t key) { if (key >= kth) { const int at = atomicAdd(&s_n, 1); if (at < Pmax) sorted[at] = key; } });
+        __syncthreads();
+        m = kc;
+    }
+    int P = 2;
+    while (P < m) P <<= 1;
+    for (int i = m + tid; i < P; i += 1024) sorted[i] = 0ull;
+    __syncthreads();
+    for (int size = 2; size <= P; size <<= 1)
+        for (int stride = size >> 1; stride > 0; stride >>= 1) {
+            for (int i = tid; i < (P >> 1); i += 1024) {
+                const int a = ((i & ~(stride - 1)) << 1) | (i & (stride - 1)), b = a + stride;
+                const bool desc = (a & size) == 0;
+                const uint64_t x = sorted[a], y = sorted[b];
+                if ((x < y) == desc) { sorted[a] = y; sorted[b] = x; }
+            }
+            __syncthreads();
+        }
+    for (int i = tid; i < kc; i += 1024) {
+        const uint64_t key = i < m ? sorted[i] : 0ull;
+        outD[q * kc + i] = key ? f32_unordered((uint32_t)(key >> 32)) : -FLT_MAX;
+        outI[q * kc + i] = key ? id_base + (int64_t)(uint32_t)(~(uint32_t)key) : -1;
     }
 }
 
 // an index that is searched without a sample: every row that is a number is a hit
 __global__ void __launch_bounds__(256)
-mx4_no_floor_kernel(int nq, float* __restrict__ tau, int64_t* __restrict__ row_below) {
+mx4_no_floor_kernel(int nq, float* __restrict__ tau, uint32_t* __restrict__ row_below) {
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i < nq) { tau[i] = -FLT_MAX; row_below[i] = 0; }
 }
