@@ -314,12 +314,13 @@ int grow_corpus_x(ipx_index* ix, int64_t need_groups, hipStream_t st) {
     return 0;
 }
 
-// Lanes per row of the mx4 row kernels, as a power of two: the most that leave at most a quarter of them idle, else those
-// that leave the fewest idle. np: pieces of eight elements per row.
-int mx4_lanes(int np, int least_l2) {
-    int best = least_l2;
+uint64_t magic_of(uint64_t by) { return by <= 1 ? 0 : ~0ull / by + 1; }       // div_by in ipx_mx4_kernels.h
+// Lanes per row of lookup_kernel, as a power of two: the most that leave at most a quarter of them idle, else those that leave
+// the fewest idle. np: pieces of eight elements per row.
+int lookup_lanes(int np) {
+    int best = 0;
     double best_use = 0.0;
-    for (int l2 = 6; l2 >= least_l2; --l2) {
+    for (int l2 = 6; l2 >= 0; --l2) {
         const int lanes = 1 << l2, turns = (np + lanes - 1) / lanes;
         const double use = (double)np / ((double)turns * lanes);
         if (use >= 0.75) return l2;
@@ -337,17 +338,16 @@ int launch_mx4_quantize(const void* rows, int dtype, int64_t n, int d, int64_t s
     const int nb = (d + 31) / 32, np = nb * 4;
     const size_t el = dtype == IPX_F32 ? 4 : 2;
     const bool wide = aligned16(rows) && stride * el % 16 == 0;
-    const int l2 = mx4_lanes(np, 2);
-    const int64_t slice = rows_per_launch(1 << l2);
+    const int64_t slice = rows_per_launch(np);
     for (int64_t r0 = 0; r0 < n; r0 += slice) {
-        const uint32_t m = (uint32_t)std::min(slice, n - r0);
+        const uint32_t total = (uint32_t)(std::min(slice, n - r0) * np);
         const void* src = (const char*)rows + (size_t)r0 * stride * el;
-        const dim3 grid((unsigned)((((int64_t)m << l2) + 255) / 256)), block(256);
+        const dim3 grid((total + 255) / 256), block(256);
         if (ix)
-            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<true>, grid, block, 0, st, src, dtype, stride, m, l2, np, d, wide,
+            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<true>, grid, block, 0, st, src, dtype, stride, total, magic_of(np), np, d, wide,
                                ix->Xx, ix->Xxs, row0 + r0, ix->nks_x, ix->nkq_x);
         else
-            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<false>, grid, block, 0, st, src, dtype, stride, m, l2, np, d, wide,
+            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<false>, grid, block, 0, st, src, dtype, stride, total, magic_of(np), np, d, wide,
                                codes + (size_t)r0 * nb * 16, scales + (size_t)r0 * nb, (int64_t)0, 0, 0);
         IPX_HIP(hipGetLastError());
     }
@@ -791,8 +791,8 @@ int scan_f32_deep(ipx_index* ix, const float* dq, const float* dw, int A, int lo
 // rescore_kernel over `nblocks` lists: 16 waves per list for the few lists of a small batch (latency), 4 otherwise.
 int launch_rescore(const ipx::RescoreParams& rp, int64_t nblocks, hipStream_t st) {
     const int dpad = rp.xfmt == 2 ? (rp.nks + 1) / 2 * 128 : rp.nks * (rp.xfmt ? 32 : 16);
-    const int fixed = ((dpad * 4 + 15) & ~15) + rp.P * 8 + (rp.P <= ipx::RS_RANK_SORT ? rp.P * 8 : 0);
-    const int per_wave = rp.xfmt == 2 ? 0 : ipx::RS_KB * 16 * ipx::RS_ROW;      // (mx4 rows are not staged)
+    const int fixed = ((dpad * 4 + 15) & ~15) + rp.P * 8 + (rp.P <= ipx::RS_RANK_SORT || rp.xfmt == 2 ? rp.P * 8 : 0);
+    const int per_wave = rp.xfmt == 2 ? 64 * ipx::RS_ROW : ipx::RS_KB * 16 * ipx::RS_ROW;
     const int nw = (nblocks <= 128 && fixed + 16 * per_wave <= 160 * 1024) ? 16 : 4;
     const int rlds = fixed + nw * per_wave;
     void (*kern)(const ipx::RescoreParams) = rp.xfmt == 2 ? (nw == 16 ? ipx::rescore_kernel<16, true> : ipx::rescore_kernel<4, true>)
@@ -1356,34 +1356,44 @@ constexpr int MX_PARTS_SCORES = 5;       // ... in ipx_scores: as exact as fp32
 constexpr int MX_MAX_K = IPX_MAX_K;      // deepest list of a search
 constexpr int MX_SLICE = 4096;           // queries per pass of a search (bounds the workspace)
 
-// How a product runs: 32-query groups per workgroup, splits of the corpus, whether the query block stays in LDS.
-struct MxGeom { int cg, nqb, S, lds; bool resident; int64_t rounds; };
-MxGeom mx4_geometry(const ipx_index* ix, int64_t nq, int quad_bytes_per_cg, int64_t ntiles) {
+// How a product runs: 32-query groups per workgroup, splits of the corpus, whether the query block stays in LDS; the
+// groups of a wave tile and the waves of a workgroup.
+#ifndef MXS_RG
+#define MXS_RG 2
+#define MXS_W 16
+#endif
+struct MxGeom { int cg, rg, waves, nqb, S, lds; bool resident; int64_t ntiles, rounds; };
+MxGeom mx4_geometry(const ipx_index* ix, int64_t nq, int quad_bytes_per_cg, int mode, int64_t groups) {
     MxGeom g;
-    const int room = 160 * 1024 - 1024, extra = 128;         // extra: hit counters, 4 bytes per query
+    const int room = 160 * 1024 - 1024;
     // the larger block (half the row traffic per product) when its queries stay in LDS; when not even 32 do (long
     // vectors), the quads go through LDS in turn
-    auto whole = [&](int cg) { return (ix->nkq_x * quad_bytes_per_cg + extra) * cg; };
-    g.cg = nq <= 32 || whole(2) > room ? 1 : 2;
-    g.resident = whole(g.cg) <= room;
+    const int whole = ix->nkq_x * quad_bytes_per_cg;
+    g.cg = nq <= 32 || 2 * whole > room ? 1 : 2;
+    g.resident = g.cg * whole <= room;
     if (!g.resident) g.cg = nq <= 32 ? 1 : 2;
-    g.lds = g.resident ? whole(g.cg) : (quad_bytes_per_cg + extra) * g.cg;
+    g.lds = g.resident ? whole * g.cg : quad_bytes_per_cg * g.cg;
+    g.rg = mode == ipx::MX_SEARCH ? 4 : MXS_RG;
+    g.waves = mode == ipx::MX_SEARCH ? 8 : g.cg == 1 ? MXS_W : 8;
     g.nqb = (int)((nq + 32 * g.cg - 1) / (32 * g.cg));
+    g.ntiles = (groups + g.rg - 1) / g.rg;
     // (a short corpus goes to as many CUs as it has tiles: a tile per wave of few workgroups leaves the matrix cores of the
     // other CUs idle — 100k x 768, one query: 19 us on 98 CUs)
-    g.S = (int)std::min<int64_t>(std::max(1, ix->num_cus / g.nqb), std::max<int64_t>(1, ntiles));
-    g.rounds = (ntiles + (int64_t)g.S * 8 - 1) / ((int64_t)g.S * 8);
+    g.S = (int)std::min<int64_t>(std::max(1, ix->num_cus / g.nqb), std::max<int64_t>(1, g.ntiles));
+    g.rounds = (g.ntiles + (int64_t)g.S * g.waves - 1) / ((int64_t)g.S * g.waves);
     return g;
 }
 
 template <int PARTS, int FMT, int MODE>
 int launch_mx4_product(const MxGeom& g, ipx::MxParams p, hipStream_t st) {
     p.S = g.S;
+    p.ntiles = g.ntiles;
+    constexpr int RG = MODE == ipx::MX_SEARCH ? 4 : MXS_RG, W1 = MODE == ipx::MX_SEARCH ? 8 : MXS_W, W2 = 8;
     void (*kern)(const ipx::MxParams) =
-        g.resident ? (g.cg == 1 ? ipx::mx4_product_kernel<1, PARTS, FMT, MODE, true> : ipx::mx4_product_kernel<2, PARTS, FMT, MODE, true>)
-                   : (g.cg == 1 ? ipx::mx4_product_kernel<1, PARTS, FMT, MODE, false> : ipx::mx4_product_kernel<2, PARTS, FMT, MODE, false>);
+        g.resident ? (g.cg == 1 ? ipx::mx4_product_kernel<1, RG, W1, PARTS, FMT, MODE, true> : ipx::mx4_product_kernel<2, RG, W2, PARTS, FMT, MODE, true>)
+                   : (g.cg == 1 ? ipx::mx4_product_kernel<1, RG, W1, PARTS, FMT, MODE, false> : ipx::mx4_product_kernel<2, RG, W2, PARTS, FMT, MODE, false>);
     if (int rc = ensure_dynamic_lds((const void*)kern, std::max(g.lds, 64 * 1024 + 1))) return rc;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(g.nqb * g.S)), dim3(ipx::MX_THREADS), g.lds, st, p);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(g.nqb * g.S)), dim3(g.waves * 64), g.lds, st, p);
     IPX_HIP(hipGetLastError());
     return 0;
 }
@@ -1397,33 +1407,41 @@ void mx4_rows(const ipx_index* ix, ipx::MxParams& p) {
     p.nkq = ix->nkq_x;
 }
 
+// margin_acc_coef for the scan of 4-bit rows: the exact chain contributes (d + 1) 2^-24. A score is the sum of nks x parts
+// MFMAs; each adds its 64 products in some order (every product takes part in one of these sums: 64 2^-24 of the sum of
+// magnitudes, at most |q||x|) to the running sum (2^-24 of it each time). Taken 4x, as there.
+float mx4_acc_coef(int d, int nks, int parts) { return (float)((d + 1 + 4.0 * (nks * parts + 64)) / 16777216.0 * 1.002); }
+
 // One search pass over the 4-bit rows: pack -> floor (from a sample) -> scan -> the kc best hits -> exact rescoring.
 // The contract of bf16_pass.
 int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* dD, int64_t* dI, hipStream_t st, bool primary,
              std::vector<int>& flagged, std::vector<int>& hard) {
     constexpr int PARTS = MX_PARTS_SEARCH, FMT = ipx::MX_E2M3;
     const int64_t N = ix->ntotal;
-    const int64_t ntiles = (N + ipx::MX_TILE - 1) / ipx::MX_TILE;
+    const int64_t groups = (N + ipx::MX_GROUP - 1) / ipx::MX_GROUP;
     const bool timing = primary && ix->timing, direct = N <= ipx::MX_DIRECT;
     const int quad1 = PARTS * ipx::mx_part_bytes<FMT>(32);
-    const MxGeom g = mx4_geometry(ix, nq, quad1, ntiles);
+    const MxGeom g = mx4_geometry(ix, nq, quad1, ipx::MX_SEARCH, groups);
     // The sample: more rows, hence a tighter floor and fewer hits, where the scores of the sample are few.
     const int m_rows = nq <= 64 && N > 2 * ipx::MX_SAMPLE_FEW ? ipx::MX_SAMPLE_FEW : ipx::MX_SAMPLE_MANY;
     // j: the wanted list's share of the sample, plus 4 standard deviations of it and a little for short lists — the list
     // comes out too short (the query is then repeated) with a probability of about 1e-5.
     const double share = (double)kc * m_rows / (double)N;
     const int j = (int)std::min<double>(m_rows, ceil(share + 4.0 * sqrt(share) + 4.0));
-    // Room per query and split: the expected hits, half as much again and 10 standard deviations; and, as all scores may be
-    // equal (a zero query: the first rows of the index are the hits), the rows of whole tiles dealt in turn.
+    // A list belongs to half a wave's rows (two per wave). Room in each: the expected hits, half as much again and 10
+    // standard deviations; and, as all scores may be equal (a zero query: the first rows of the index are the hits), half
+    // the rows of as many tiles as those rows give a wave.
     const double hits = (double)j * (double)N / m_rows;
-    const int64_t split_rows = (ntiles + g.S - 1) / g.S * ipx::MX_TILE, turn_rows = ((int64_t)(hits / ipx::MX_TILE / g.S) + 2) * ipx::MX_TILE;
-    const int64_t cap = direct ? split_rows
-                               : std::min<int64_t>(split_rows, std::max<int64_t>(turn_rows, (int64_t)(1.5 * hits / g.S + 10.0 * sqrt(hits / g.S)) + 32));
+    const int64_t waves = (int64_t)g.S * g.waves, nlists = 2 * waves;
+    const int64_t tile_half = g.rg * ipx::MX_GROUP / 2, all = g.rounds * tile_half;
+    const int64_t first_rows = ((int64_t)((hits + 64) / (2 * tile_half)) / waves + 1) * tile_half;
+    const int64_t want = direct ? all : std::min<int64_t>(all, std::max<int64_t>(first_rows, (int64_t)(1.5 * hits / nlists + 10.0 * sqrt(hits / nlists)) + 8));
+    const int64_t cap = std::min<int64_t>(want, (int64_t)0xffff0000u / (32 * g.cg * nlists * 8));      // (32-bit offsets in the kernel)
     const size_t info_bytes = ((size_t)nq * sizeof(ipx::MxQueryInfo) + 255) / 256 * 256, word = ((size_t)nq * 4 + 255) / 256 * 256;
 
     if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
-    if (int rc = ix->cand.ensure((size_t)nq * g.S * cap * sizeof(uint64_t))) return rc;
-    if (int rc = ix->deepN.ensure((size_t)nq * g.S * sizeof(int))) return rc;
+    if (int rc = ix->cand.ensure((size_t)nq * nlists * cap * sizeof(uint2))) return rc;
+    if (int rc = ix->deepN.ensure((size_t)nq * nlists * sizeof(int))) return rc;
     if (int rc = ix->candD.ensure((size_t)nq * kc * sizeof(float))) return rc;
     if (int rc = ix->candI.ensure((size_t)nq * kc * sizeof(int64_t))) return rc;
     if (int rc = ix->mxq.ensure(info_bytes + 3 * word)) return rc;         // norms, row bounds, floors, list states
@@ -1437,7 +1455,8 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
 
     if (timing) IPX_HIP(hipEventRecord(ix->ev[0], st));
     hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)(g.nqb * 32 * g.cg)), dim3(256), 0, st, (const void*)qf,
-                       (int)IPX_F32, (int)nq, ix->d, PARTS, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, info, todo);
+                       (int)IPX_F32, (int)nq, ix->d, PARTS, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, info, todo,
+                       direct ? tau : nullptr, below);
     IPX_HIP(hipGetLastError());
     ipx::MxParams p = {};
     mx4_rows(ix, p);
@@ -1445,40 +1464,34 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     p.nq = (int)nq;
     p.q_dtype = IPX_F32;
     p.info = info;
-    if (direct) {
-        hipLaunchKernelGGL(ipx::mx4_no_floor_kernel, dim3((unsigned)((nq + 255) / 256)), dim3(256), 0, st, (int)nq, tau, below);
-        IPX_HIP(hipGetLastError());
-    } else {
+    if (!direct) {
         ipx::MxParams ps = p;
-        ps.ntiles = m_rows / ipx::MX_TILE;
-        ps.gstep = (N / ipx::MX_GROUP - ipx::MX_RG) / (ps.ntiles - 1);      // whole groups, spread over the index
+        const MxGeom gs = mx4_geometry(ix, nq, quad1, ipx::MX_SCORES, m_rows / ipx::MX_GROUP);
+        ps.gstep = (N / ipx::MX_GROUP - gs.rg) / (gs.ntiles - 1);      // whole groups, spread over the index
         ps.out = (float*)ix->mxs.p;
         ps.ld = m_rows;
         ps.row0 = -1;
         ps.n = m_rows;
-        MxGeom gs = g;
-        gs.S = (int)std::min<int64_t>(g.S, ps.ntiles);
         if (int rc = launch_mx4_product<PARTS, FMT, ipx::MX_SCORES>(gs, ps, st)) return rc;
         hipLaunchKernelGGL((m_rows == ipx::MX_SAMPLE_FEW ? ipx::mx4_floor_kernel<ipx::MX_SAMPLE_FEW / 1024> : ipx::mx4_floor_kernel<ipx::MX_SAMPLE_MANY / 1024>),
                            dim3((unsigned)nq), dim3(1024), 0, st, (const float*)ix->mxs.p, j, N, tau, below);
         IPX_HIP(hipGetLastError());
     }
     if (timing) IPX_HIP(hipEventRecord(ix->ev[1], st));
-    p.gstep = ipx::MX_RG;
-    p.ntiles = ntiles;
+    p.gstep = g.rg;
     p.tau = tau;
     p.row_below = below;
-    p.cand = (uint64_t*)ix->cand.p;
+    p.cand = (uint2*)ix->cand.p;
     p.cnt = (int*)ix->deepN.p;
     p.todo = todo;
     p.cap = (int)cap;
     if (int rc = launch_mx4_product<PARTS, FMT, ipx::MX_SEARCH>(g, p, st)) return rc;
     if (timing) IPX_HIP(hipEventRecord(ix->ev[2], st));
     const int Pmax = next_pow2(std::max(512, kc + kc / 4));
-    const int slds = (Pmax + ipx::MX_HELD) * 8 + g.S * 4;
+    const int slds = (Pmax + ipx::MX_HELD) * 8;
     if (int rc = ensure_dynamic_lds((const void*)ipx::mx4_select_kernel, std::max(slds, 64 * 1024 + 1))) return rc;
-    hipLaunchKernelGGL(ipx::mx4_select_kernel, dim3((unsigned)nq), dim3(1024), slds, st, (const uint64_t*)ix->cand.p,
-                       (const int*)ix->deepN.p, g.S, (int)cap, kc, Pmax, ix->id_base, (float*)ix->candD.p, (int64_t*)ix->candI.p);
+    hipLaunchKernelGGL(ipx::mx4_select_kernel, dim3((unsigned)nq), dim3(1024), slds, st, (const uint2*)ix->cand.p,
+                       (const int*)ix->deepN.p, (int)nlists, (int)cap, kc, Pmax, ix->id_base, (float*)ix->candD.p, (int64_t*)ix->candI.p);
     IPX_HIP(hipGetLastError());
     if (timing) {
         IPX_HIP(hipEventRecord(ix->ev[3], st));
@@ -1501,7 +1514,7 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     rp.shared_list = 0;
     rp.nq = (int)nq;
     rp.id_base = ix->id_base;
-    rp.acc_coef = margin_acc_coef(ix->nks_x * ipx::MX_KSET, PARTS);
+    rp.acc_coef = mx4_acc_coef(ix->d, ix->nks_x, PARTS);
     rp.qparts = PARTS;
     rp.post = ix->margin_post;
     rp.d = ix->d;
@@ -1535,7 +1548,10 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
     const float* qf = dq;
     if (A > 0)
         if (int rc = fuse_queries(ix, dq, dw, A, logits, nq, st, &qf)) return rc;
-    const int kc0 = ix->force_kc > 0 ? ix->force_kc : std::max(128, k + k / 2);
+    // The list has to reach e below the k-th score (rescore_kernel, post): 1.8M Gaussian rows of 768, k = 100: 120 left 2 of
+    // 64 queries to the repeat pass, 125 none; 500k, k = 1000: 1100 left 131 of 1000, 1150 none. Rows whose norms spread
+    // widen e: the list then grows as in the bf16 scan (ipx_index::kc_boost).
+    const int kc0 = ix->force_kc > 0 ? ix->force_kc : (int)((int64_t)std::max(128, k + k / 4) * ix->kc_boost / 8);
     const int kc = std::min(std::max(kc0, k), MAX_KC);
     for (int64_t q0 = 0; q0 < nq; q0 += MX_SLICE) {
         const int64_t n = std::min<int64_t>(MX_SLICE, nq - q0);
@@ -1545,6 +1561,8 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
         std::vector<int> flagged, hard;
         if (int rc = mx4_pass(ix, q, n, k, kc, D, I, st, q0 == 0, flagged, hard)) return rc;
         ix->last_fallback += (int64_t)(flagged.size() + hard.size());
+        if (ix->force_kc == 0 && n >= 64 && kc < MAX_KC && (int64_t)flagged.size() * 1000 > n)
+            ix->kc_boost = std::min(128, ix->kc_boost + (ix->kc_boost + 3) / 4);
         if (!flagged.empty()) {
             std::vector<int> still, still_hard;
             int rc = redo_queries(ix, q, flagged, k, D, I, st, [&](const float* q2, int64_t n2, float* D2, int64_t* I2) {
@@ -1562,7 +1580,8 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
         if (int rc = ix->Qp.ensure((size_t)((n + 31) / 32) * ix->nkq_x * ipx::mx_part_bytes<ipx::MX_E2M3>(32))) return rc;
         if (int rc = ix->mxq.ensure((size_t)n * sizeof(ipx::MxQueryInfo))) return rc;
         hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)n), dim3(256), 0, st, (const void*)q, (int)IPX_F32, (int)n,
-                           ix->d, 1, 32, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr);
+                           ix->d, 1, 32, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr,
+                       (float*)nullptr, (uint32_t*)nullptr);
         IPX_HIP(hipGetLastError());
         if (int rc = exact_rows_path(ix, q, hard, k, D, I, st)) return rc;
     }
@@ -1574,9 +1593,10 @@ int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sca
                 hipStream_t st) {
     ipx::MxParams p = {};
     mx4_rows(ix, p);
-    p.g0 = row0 / ipx::MX_TILE * ipx::MX_RG;             // whole tiles: the buffers end behind one
-    p.gstep = ipx::MX_RG;
-    p.ntiles = (row0 + n + ipx::MX_TILE - 1) / ipx::MX_TILE - row0 / ipx::MX_TILE;
+    // (a tile is a power of two of groups and the buffers end behind eight: groups up to a tile's end exist)
+    p.g0 = row0 / ipx::MX_GROUP / MXS_RG * MXS_RG;
+    p.gstep = MXS_RG;
+    const int64_t groups = (row0 + n + ipx::MX_GROUP - 1) / ipx::MX_GROUP - p.g0;
     p.nq = (int)nq;
     p.out = out;
     p.ld = n;
@@ -1584,7 +1604,7 @@ int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sca
     p.n = n;
     if (q_scales) {
         const int quad1 = ipx::mx_part_bytes<ipx::MX_E2M1>(32);
-        const MxGeom g = mx4_geometry(ix, nq, quad1, p.ntiles);
+        const MxGeom g = mx4_geometry(ix, nq, quad1, ipx::MX_SCORES, groups);
         if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
         const int64_t total = (int64_t)g.nqb * 32 * g.cg * ix->nkq_x * 8;
         hipLaunchKernelGGL(ipx::mx4_pack_codes_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, (const uint8_t*)dq,
@@ -1594,11 +1614,12 @@ int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sca
         return launch_mx4_product<1, ipx::MX_E2M1, ipx::MX_SCORES>(g, p, st);
     }
     const int quad1 = MX_PARTS_SCORES * ipx::mx_part_bytes<ipx::MX_E2M3>(32);
-    const MxGeom g = mx4_geometry(ix, nq, quad1, p.ntiles);
+    const MxGeom g = mx4_geometry(ix, nq, quad1, ipx::MX_SCORES, groups);
     if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
     if (int rc = ix->mxq.ensure((size_t)nq * sizeof(ipx::MxQueryInfo))) return rc;
     hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)(g.nqb * 32 * g.cg)), dim3(256), 0, st, dq, q_dtype, (int)nq,
-                       ix->d, MX_PARTS_SCORES, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr);
+                       ix->d, MX_PARTS_SCORES, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr,
+                       (float*)nullptr, (uint32_t*)nullptr);
     IPX_HIP(hipGetLastError());
     p.Q = (const uint8_t*)ix->Qp.p;
     p.q = dq;
@@ -1946,6 +1967,7 @@ int ipx_add_mx4(ipx_index* ix, const uint8_t* codes, const uint8_t* scales, int6
     if (ix->ntotal + n > (int64_t)0x7fffff00) return fail(IPX_ERR_ARG, "add_mx4: more than 2^31 rows in one index");
     IPX_ON_DEVICE(ix->device);
     hipStream_t st = (hipStream_t)stream;
+    ix->kc_boost = 8;                     // new rows, new norm bound
     if (int rc = grow_storage(ix, ix->ntotal + n, st)) return rc;
     const int nb = (ix->d + 31) / 32;
     // host rows travel in slices of 256 MiB
@@ -1983,6 +2005,7 @@ static int scores_impl(ipx_index* ix, const char* who, const void* q, int q_dtyp
     if (row0 < 0 || n < 0 || row0 > ix->ntotal || n > ix->ntotal - row0)
         return fail(IPX_ERR_ARG, w + ": rows [" + std::to_string(row0) + ", " + std::to_string(row0) + " + " + std::to_string(n) +
                     ") outside the index of " + std::to_string(ix->ntotal));
+    if (n >= (1 << 27)) return fail(IPX_ERR_ARG, w + ": n=" + std::to_string(n) + ": 2^27 rows and more take several calls");
     if (nq == 0 || n == 0) return 0;
     if (!q || !out || (mx4 && !q_scales)) return fail(IPX_ERR_ARG, w + ": null pointer");
     IPX_ON_DEVICE(ix->device);
@@ -2046,7 +2069,7 @@ int ipx_lookup(ipx_index* ix, const int64_t* ids, int64_t n, const float* scale,
     const void* X = xfmt == 2 ? (const void*)ix->Xx : xfmt ? (const void*)ix->Xh : (const void*)ix->Xp;
     const int nks = xfmt == 2 ? ix->nks_x : xfmt ? ix->nks_h : ix->nks;
     const bool wide = aligned16(dout) && row_bytes % 16 == 0;
-    const int l2 = mx4_lanes(np, 0);
+    const int l2 = lookup_lanes(np);
     const int64_t slice = rows_per_launch(1 << l2);
     auto kern = xfmt == 2 ? ipx::lookup_kernel<2> : xfmt == 1 ? ipx::lookup_kernel<1> : ipx::lookup_kernel<0>;
     for (int64_t i0 = 0; i0 < n; i0 += slice) {
@@ -2122,12 +2145,11 @@ int ipx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n, i
     const int np = (d + 7) / 8;
     // (the wide form also reads the codes as dwords: they then start at a multiple of 4 bytes)
     const bool wide = aligned16(dout) && row_bytes % 16 == 0 && ((uintptr_t)dc & 3) == 0;
-    const int l2 = mx4_lanes(np, 0);
-    const int64_t slice = rows_per_launch(1 << l2);
+    const int64_t slice = rows_per_launch(np);
     for (int64_t r0 = 0; r0 < n && e == hipSuccess; r0 += slice) {
-        const uint32_t m = (uint32_t)std::min(slice, n - r0);
-        hipLaunchKernelGGL(ipx::mx4_dequantize_kernel, dim3((unsigned)((((int64_t)m << l2) + 255) / 256)), dim3(256), 0, st,
-                           dc + (size_t)r0 * nb * 16, ds + (size_t)r0 * nb, m, l2, np, d, (int)nb, (void*)(dout + (size_t)r0 * row_bytes), dtype, wide);
+        const uint32_t total = (uint32_t)(std::min(slice, n - r0) * np);
+        hipLaunchKernelGGL(ipx::mx4_dequantize_kernel, dim3((total + 255) / 256), dim3(256), 0, st, dc + (size_t)r0 * nb * 16,
+                           ds + (size_t)r0 * nb, total, magic_of(np), np, d, (int)nb, (void*)(dout + (size_t)r0 * row_bytes), dtype, wide);
         e = hipGetLastError();
     }
     if (!on_device) {

@@ -929,6 +929,67 @@ constexpr int RS_RANK_SORT = 1024;   // lists of up to this many scored candidat
 // NW waves per query: 4 for large batches (the chip is full of workgroups anyway), 16 for small ones, where a query's
 // workgroup is alone on its CU and the time is the latency of its dependent rounds — 256 candidates in flight per
 // round instead of 64. The rows' K-stages are fetched one group ahead of the fmaf chains that consume them.
+// Places of the keys (m slots in LDS, 0: none) in descending order, without a sort: a histogram of the scores between the
+// lowest and the best, linear in their bits, gives a key its step's place; there it counts the larger keys of its own step.
+// emit(place, key) once per key; returns how many there are. steps: 2 x 2048 ints of LDS. (2048 slots sorted by 256 threads
+// took two thirds of the rescoring of 1000 x 1500 candidates: 66 rounds of exchanges.)
+template <int NT, class F>
+__device__ __forceinline__ int place_in_steps(const uint64_t* keys, int m, uint64_t* placed, int* steps, F emit) {
+    constexpr int NW = NT / 64, PER = 2048 / NT;
+    __shared__ uint32_t s_lo[NW], s_hi[NW];
+    __shared__ int s_sum[NW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int *first = steps, *fill = steps + 2048;
+    uint32_t lo = 0xffffffffu, hi = 0;
+    for (int i = tid; i < m; i += NT) {
+        const uint32_t v = (uint32_t)(keys[i] >> 32);
+        if (v) { lo = min(lo, v); hi = max(hi, v); }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        lo = min(lo, (uint32_t)__shfl_xor((int)lo, o));
+        hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
+    }
+    if (lane == 0) { s_lo[wave] = lo; s_hi[wave] = hi; }
+    for (int i = tid; i < 4096; i += NT) steps[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) { lo = min(lo, s_lo[w]); hi = max(hi, s_hi[w]); }
+    const int shift = hi ? max(0, 21 - __clz((int)((hi - lo) | 1u))) : 0;           // (hi - lo) >> shift < 2048
+    for (int i = tid; i < m; i += NT)
+        if (keys[i]) atomicAdd(&first[(hi - (uint32_t)(keys[i] >> 32)) >> shift], 1);
+    __syncthreads();
+    int mine = 0;
+#pragma unroll
+    for (int u = 0; u < PER; ++u) mine += first[tid * PER + u];
+    int run = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(run, o); if (lane >= o) run += y; }
+    if (lane == 63) s_sum[wave] = run;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) { if (w < wave) run += s_sum[w]; total += s_sum[w]; }
+    int before = run - mine;
+#pragma unroll
+    for (int u = 0; u < PER; ++u) { const int n = first[tid * PER + u]; first[tid * PER + u] = before; before += n; }
+    __syncthreads();
+    for (int i = tid; i < m; i += NT)
+        if (const uint64_t key = keys[i]) {
+            const int b = (int)((hi - (uint32_t)(key >> 32)) >> shift);
+            placed[first[b] + atomicAdd(&fill[b], 1)] = key;
+        }
+    __syncthreads();
+    for (int i = tid; i < total; i += NT) {
+        const uint64_t key = placed[i];
+        const int b = (int)((hi - (uint32_t)(key >> 32)) >> shift), from = first[b], to = from + fill[b];
+        int at = from;
+        for (int x = from; x < to; ++x) at += placed[x] > key ? 1 : 0;
+        emit(at, key);
+    }
+    return total;
+}
+
 template <int NW, bool MX4 = false>
 __global__ void __launch_bounds__(NW * 64)
 rescore_kernel(const RescoreParams p) {
@@ -1047,41 +1108,52 @@ rescore_kernel(const RescoreParams p) {
     for (int i = tid; i < p.P; i += NT) keys[i] = 0;
     __syncthreads();            // a wave writes keys that other waves' threads cleared
     // short lists are sorted by rank (one pass, no barriers inside) into a second array behind the first
-    const bool by_rank = p.P <= RS_RANK_SORT;
+    const bool by_rank = MX4 || p.P <= RS_RANK_SORT;
     uint64_t* sorted = keys + p.P;                            // [P] when by_rank
     char* stage = (char*)(sorted + (by_rank ? p.P : 0)) + wave * (RS_KB * 16 * RS_ROW);
     if constexpr (MX4) {
         // mx4 rows: 64 candidates per wave, one per lane — the chain of a candidate is serial, so the lanes are what there is
-        // to fill (four lanes to a row and 16 chains a wave took 360 us for 1000 x 1500 candidates of 768). A lane fetches
-        // its own row, 64 bytes (128 elements, two K-sets) at a time, one line ahead, and its scales, one quad ahead. Values
-        // are exact in fp32, so the chain is the one a bf16 index of these values runs.
+        // to fill (16 chains a wave took 360 us for 1000 x 1500 candidates of 768). Rows come 64 bytes (128 elements, two
+        // K-sets) at a time, one line ahead, four lanes to a line (every lane its own line: each of a line's four loads
+        // misses), and reach their lanes through LDS; a lane fetches its own scales, one quad ahead. Values are exact in
+        // fp32, so the chain is the one a bf16 index of these values runs.
         const int nb = (p.d + 31) / 32, nlines = (p.nks + 1) / 2;
+        char* lines = (char*)(sorted + (by_rank ? p.P : 0)) + wave * (64 * RS_ROW);
         for (int g0 = wave * 64; g0 < m; g0 += NT) {
             const int my = g0 + lane < m ? g0 + lane : m - 1;
             const int64_t row = cI[my] - p.id_base;
-            const uint8_t* src = (const uint8_t*)p.X + (size_t)(row >> 5) * p.nks * 1024;
-            const int rr = (int)(row & 31);
             const uint2* sp = (const uint2*)(p.Xs + (size_t)row * p.nkq * 8);
-            float acc = 0.f;
-            uint4 v[4];
+            // lane 4 r + c fetches piece c of the lines of candidates r, 16 + r, 32 + r, 48 + r
             // (ipx_mx4_kernels.h, mx_code_at: a last K-set without a partner lies in 32-byte pieces; its line is read twice
             // over, the second half is not used)
-            auto fetch = [&](int line) {
-                line = line < nlines ? line : nlines - 1;
-                const bool alone = 2 * line + 1 == p.nks;
-                const uint4* at = (const uint4*)(src + line * 2048 + (alone ? rr * 32 : rr * 64));
-                v[0] = at[0];
-                v[1] = at[1];
-                v[2] = at[alone ? 0 : 2];
-                v[3] = at[alone ? 1 : 3];
+            // (named registers, not arrays: hipcc keeps an array that is live across the loop in scratch memory)
+            const bool odd = p.nks & 1;
+            auto place = [&](int i, int& last) {              // candidate i * 16 + r: its first line; from there to its last
+                const int who = i * 16 + (lane >> 2);
+                const int64_t other = cI[g0 + who < m ? g0 + who : m - 1] - p.id_base;
+                const int at = (int)(other & 31) * 64 + (lane & 3) * 16, alone = (int)(other & 31) * 32 + (lane & 1) * 16;
+                last = (nlines - 1) * 2048 + (odd ? alone - at : 0);
+                return (const uint8_t*)p.X + (size_t)(other >> 5) * p.nks * 1024 + at;
             };
-            fetch(0);
+            int e0, e1, e2, e3;
+            const uint8_t *x0 = place(0, e0), *x1 = place(1, e1), *x2 = place(2, e2), *x3 = place(3, e3);
+            float acc = 0.f;
+            auto fetch = [&](const uint8_t* x, int line, int last) { return *(const uint4*)(x + (line < nlines - 1 ? line * 2048 : last)); };
+            uint4 v0 = fetch(x0, 0, e0), v1 = fetch(x1, 0, e1), v2 = fetch(x2, 0, e2), v3 = fetch(x3, 0, e3);
             uint2 sc = sp[0];
             for (int line = 0; line < nlines; ++line) {
-                const uint4 c[4] = {v[0], v[1], v[2], v[3]};
+                wave_lds_sync();
+                char* to = lines + (lane >> 2) * RS_ROW + (lane & 3) * 16;
+                *(uint4*)(to) = v0;
+                *(uint4*)(to + 16 * RS_ROW) = v1;
+                *(uint4*)(to + 32 * RS_ROW) = v2;
+                *(uint4*)(to + 48 * RS_ROW) = v3;
+                v0 = fetch(x0, line + 1, e0); v1 = fetch(x1, line + 1, e1); v2 = fetch(x2, line + 1, e2); v3 = fetch(x3, line + 1, e3);
+                wave_lds_sync();
+                const uint4* own = (const uint4*)(lines + lane * RS_ROW);
+                const uint4 c[4] = {own[0], own[1], own[2], own[3]};
                 const uint32_t two = (line & 1) * 16;                       // this line's scale bytes of the quad
                 const uint32_t s0 = sc.x >> two, s1 = sc.y >> two;
-                fetch(line + 1);
                 if (line & 1) sc = sp[(line + 1) / 2 < p.nkq ? (line + 1) / 2 : p.nkq - 1];
                 const int blocks = nb - line * 4;                           // 4 except in the last line
 #pragma unroll
@@ -1165,6 +1237,20 @@ rescore_kernel(const RescoreParams p) {
     }
     }
     __syncthreads();
+    if constexpr (MX4) {
+        const int n = place_in_steps<NT>(keys, m, sorted, (int*)(sorted + p.P), [&](int at, uint64_t key) {
+            const float score = f32_unordered((uint32_t)(key >> 32));
+            if (at == p.k - 1 && s_post && cD[p.kc - 1] + eps < score) p.flags[qi] = 0;
+            if (at >= p.k) return;
+            p.outD[qi * p.k + at] = score;
+            p.outI[qi * p.k + at] = p.id_base + (int64_t)(uint32_t)(~(uint32_t)key);
+        });
+        for (int i = n + tid; i < p.k; i += NT) {
+            p.outD[qi * p.k + i] = -FLT_MAX;
+            p.outI[qi * p.k + i] = -1;
+        }
+        return;
+    }
     const uint64_t* res = keys;
     if (by_rank) {
         // rank of a key = how many keys are larger (distinct rows: distinct keys; the zeros of rows that were not

@@ -35,9 +35,6 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int MX_GROUP = 32;             // rows per group
 constexpr int MX_KSET = 64;              // elements per K-set
 constexpr int MX_SET_BYTES = 1024;       // codes of one K-set of one group
-constexpr int MX_THREADS = 512;          // 8 waves
-constexpr int MX_RG = 4;                 // groups per wave tile
-constexpr int MX_TILE = MX_RG * MX_GROUP;
 constexpr int MX_SAMPLE_FEW = 32768;     // rows a search samples for its floor: few queries (mx4_floor_kernel)
 constexpr int MX_SAMPLE_MANY = 8192;     // ... many
 constexpr int MX_DIRECT = 16384;         // indexes of up to this many rows are searched without a floor (fewer than the sample: neither)
@@ -108,20 +105,25 @@ __device__ __forceinline__ void store8(void* out, int dtype, size_t i, const flo
         }
 }
 
-// The row kernels below give a row 2^l2 adjacent lanes, each of which takes every 2^l2-th piece of eight elements; the host
-// picks the l2 that leaves the fewest lanes idle (mx4_lanes).
+// Quantisation and dequantisation take one piece of eight elements per thread, in the order of memory: a linear sweep of the whole chip
+// writes at 6.6-7 TB/s, where workgroups that each walk their own stretch reach 4.6 (1 GiB).
+__device__ __forceinline__ uint32_t div_by(uint32_t i, uint64_t magic) {      // i / by, magic = ceil(2^64 / by), by > 1
+    return (uint32_t)__umul64hi((uint64_t)i, magic);
+}
 
 // ---- quantisation ----------------------------------------------------------------------------------------------
 // Rows [n, d] (f32 / f16 / bf16, `stride` elements apart) -> codes and scales, in the external form or (INDEX) at rows
-// row0.. of an index. Four adjacent lanes per block, eight elements each (2^l2 >= 4): the block's largest magnitude is two
-// exchanges of lanes away. Bound by HBM.
+// row0.. of an index. Four adjacent lanes per block, eight elements each: the block's largest magnitude is two exchanges of
+// lanes away. Bound by HBM.
 template <bool INDEX>
 __global__ void __launch_bounds__(256)
-mx4_quantize_kernel(const void* __restrict__ src, int dtype, int64_t stride, uint32_t n, int l2, int np, int d, bool wide,
+mx4_quantize_kernel(const void* __restrict__ src, int dtype, int64_t stride, uint32_t total, uint64_t magic, int np, int d, bool wide,
                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t row0, int nks, int nkq) {
-    const uint32_t gid = blockIdx.x * 256u + threadIdx.x, r = gid >> l2;
-    if (r >= n) return;
-    for (int piece = (int)(gid & ((1u << l2) - 1)); piece < np; piece += 1 << l2) {
+    const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
+    if (gid >= total) return;                               // a multiple of 4: the four lanes of a block stay together
+    const uint32_t r = div_by(gid, magic);
+    const int piece = (int)(gid - r * (uint32_t)np);
+    {
         const int e0 = piece * 8;
         const int64_t at = (int64_t)r * stride + e0;
         float x[8];
@@ -189,18 +191,18 @@ mx4_place_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ 
 
 // external form -> values
 __global__ void __launch_bounds__(256)
-mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t n, int l2, int np, int d, int nb,
-                      void* __restrict__ out, int dtype, bool wide) {
-    const uint32_t gid = blockIdx.x * 256u + threadIdx.x, r = gid >> l2;
-    if (r >= n) return;
-    for (int piece = (int)(gid & ((1u << l2) - 1)); piece < np; piece += 1 << l2) {
-        const size_t blk = (size_t)r * nb + (piece >> 2);
-        const uint8_t* s = codes + blk * 16 + (piece & 3) * 4;
-        const uint32_t w = wide ? *(const uint32_t*)s : s[0] | (uint32_t)s[1] << 8 | (uint32_t)s[2] << 16 | (uint32_t)s[3] << 24;
-        float v[8];
-        mx_decode8(w, scales[blk], v);
-        store8(out, dtype, (size_t)r * d + piece * 8, v, d - piece * 8, wide);
-    }
+mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t total, uint64_t magic, int np,
+                      int d, int nb, void* __restrict__ out, int dtype, bool wide) {
+    const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
+    if (gid >= total) return;
+    const uint32_t r = np == 1 ? gid : div_by(gid, magic);
+    const int piece = (int)(gid - r * (uint32_t)np);
+    const size_t blk = (size_t)r * nb + (piece >> 2);
+    const uint8_t* s = codes + blk * 16 + (piece & 3) * 4;
+    const uint32_t w = wide ? *(const uint32_t*)s : s[0] | (uint32_t)s[1] << 8 | (uint32_t)s[2] << 16 | (uint32_t)s[3] << 24;
+    float v[8];
+    mx_decode8(w, scales[blk], v);
+    store8(out, dtype, (size_t)r * d + piece * 8, v, d - piece * 8, wide);
 }
 
 // max |x|^2 over rows [row0, row0 + n) of an mx4 index, for the margin rule (rescore_kernel), as float bits. A row with a
@@ -239,12 +241,16 @@ mx4_norm_max_kernel(const uint8_t* __restrict__ X, const uint8_t* __restrict__ X
 // ---- lookup ----------------------------------------------------------------------------------------------------
 // out[i] = scale[i] * row(ids[i]) for an index of any storage (XFMT 0: fp32 tiles of 128 rows, 1: bf16 tiles of 256, 2: mx4).
 // The product is rounded to fp32, then once to the output type. The empty slot id -1 gives a row of zeros; so does any other
-// id outside the index, which also sets *err.
+// id outside the index, which also sets *err. A row has 2^l2 adjacent lanes, each with several pieces of eight elements (the
+// host leaves the fewest lanes idle: lookup_lanes): a row's address takes two dependent loads, one piece per lane was bound
+// by them (698k rows of 768 out of 1.8M, bf16 out: 480 us; so 366). Rows are gathered in 64-byte pieces, for which the
+// memory moves 128 bytes: 0.9 KB per mx4 row of 768 elements, that and the output at 4.6 TB/s.
 template <int XFMT>
 __global__ void __launch_bounds__(256)
 lookup_kernel(const void* __restrict__ X, const uint8_t* __restrict__ Xs, int nks, int nkq, int64_t id_base, int64_t N,
               const int64_t* __restrict__ ids, const float* __restrict__ scale, uint32_t n, int l2, int np, int d,
               void* __restrict__ out, int dtype, bool wide, int* err) {
+    constexpr int AHEAD = 4;                                   // pieces a lane has in flight
     const uint32_t gid = blockIdx.x * 256u + threadIdx.x, i = gid >> l2;
     if (i >= n) return;
     const int64_t id = ids[i];
@@ -253,33 +259,48 @@ lookup_kernel(const void* __restrict__ X, const uint8_t* __restrict__ Xs, int nk
     const bool have = row < (uint64_t)N;
     const int first = (int)(gid & ((1u << l2) - 1));
     if (!have && id != -1 && first == 0) *err = 1;
-    for (int piece = first; piece < np; piece += 1 << l2) {
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (have) {
+    for (int p0 = first; p0 < np; p0 += AHEAD << l2) {
+        uint4 w[AHEAD] = {}, w2[AHEAD] = {};                   // mx4: codes and scale byte; bf16: w; fp32: both
+        if (have)
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int piece = min(p0 + (u << l2), np - 1);
+                if constexpr (XFMT == 2) {
+                    const int b = piece >> 2;
+                    w[u].x = *(const uint32_t*)((const uint8_t*)X + mx_code_at((int64_t)row, b, nks) + (piece & 3) * 4);
+                    w[u].y = Xs[mx_scale_at((int64_t)row, b, nkq)];
+                } else if constexpr (XFMT == 1) {
+                    const int64_t tile = (int64_t)row / HBD;
+                    const int rr = (int)(row - (uint64_t)tile * HBD), c = (piece & 3) ^ ((rr >> 2) & 3);
+                    w[u] = *(const uint4*)((const char*)X + (((size_t)tile * nks + (piece >> 2)) * HBD + rr) * 64 + c * 16);
+                } else {
+                    const int64_t tile = (int64_t)row / BD;
+                    const int rr = (int)(row - (uint64_t)tile * BD), sw = (rr >> 2) & 3, c0 = (piece & 1) * 2;
+                    const char* line = (const char*)X + (((size_t)tile * nks + (piece >> 1)) * BD + rr) * 64;
+                    w[u] = *(const uint4*)(line + (c0 ^ sw) * 16);
+                    w2[u] = *(const uint4*)(line + ((c0 + 1) ^ sw) * 16);
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int piece = p0 + (u << l2);
+            if (piece >= np) break;
+            float v[8];
+            const uint32_t ws[8] = {w[u].x, w[u].y, w[u].z, w[u].w, w2[u].x, w2[u].y, w2[u].z, w2[u].w};
             if constexpr (XFMT == 2) {
-                const int b = piece >> 2;
-                const uint32_t w = *(const uint32_t*)((const uint8_t*)X + mx_code_at((int64_t)row, b, nks) + (piece & 3) * 4);
-                mx_decode8(w, Xs[mx_scale_at((int64_t)row, b, nkq)], v);
+                mx_decode8(ws[0], ws[1], v);
             } else if constexpr (XFMT == 1) {
-                const int64_t tile = (int64_t)row / HBD;
-                const int rr = (int)(row - (uint64_t)tile * HBD), c = (piece & 3) ^ ((rr >> 2) & 3);
-                const uint4 w = *(const uint4*)((const char*)X + (((size_t)tile * nks + (piece >> 2)) * HBD + rr) * 64 + c * 16);
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { v[2 * e] = bf16_lo(ws[e]); v[2 * e + 1] = bf16_hi(ws[e]); }
             } else {
-                const int64_t tile = (int64_t)row / BD;
-                const int rr = (int)(row - (uint64_t)tile * BD), sw = (rr >> 2) & 3, c0 = (piece & 1) * 2;
-                const char* line = (const char*)X + (((size_t)tile * nks + (piece >> 1)) * BD + rr) * 64;
-                const f32x4 a = *(const f32x4*)(line + (c0 ^ sw) * 16), b = *(const f32x4*)(line + ((c0 + 1) ^ sw) * 16);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(ws[e]);
             }
-            if (scale)
+            if (scale && have)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= s;
+            store8(out, dtype, (size_t)i * d + piece * 8, v, d - piece * 8, wide);
         }
-        store8(out, dtype, (size_t)i * d + piece * 8, v, d - piece * 8, wide);
     }
 }
 
@@ -298,10 +319,11 @@ struct MxQueryInfo {      // of one query
     float restsq;         // |q - sum of its parts|^2        very small elements vanish, the bounds they stand for must not)
 };
 
-// One workgroup per query (rows beyond nq are written as zeros). Eight lanes per block, four elements each.
+// One workgroup per query (rows beyond nq are written as zeros). Eight lanes per block, four elements each. With `tau`, the
+// state of a search without a floor is written too: every row that scores a number is a hit.
 __global__ void __launch_bounds__(256)
 mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, int parts, int bq, int nkq, uint8_t* __restrict__ dst,
-                        MxQueryInfo* __restrict__ info, int* __restrict__ todo) {
+                        MxQueryInfo* __restrict__ info, int* __restrict__ todo, float* __restrict__ tau, uint32_t* __restrict__ row_below) {
     __shared__ float red[8];
     const int tid = threadIdx.x, lane = tid & 63;
     bool nonzero = false;
@@ -324,27 +346,24 @@ mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, 
             uint32_t top = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-#pragma unroll
-            for (int off = 1; off < 8; off <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));       // quad_perm [1,0,3,2]
+            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));       // quad_perm [2,3,0,1]
+            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xF, 0xF, true));      // row_half_mirror
             const bool bad = top >= 0x7f800000u;                        // NaN / inf: the block's scale is NaN
-            // smallest s with the largest magnitude <= 7.5 x 2^s
-            int s = -127;
-            if (!bad && top) {
-                int ex;
-                const float m = frexpf(__uint_as_float(top), &ex);      // m 2^ex, 0.5 <= m < 1
-                s = max(ex - 3 + (m > 0.9375f ? 1 : 0), -127);
-            }
+            // smallest s in [-127, 125] with the largest magnitude <= 7.5 x 2^s
+            const int s = max((int)(top >> 23) - 129 + ((top & 0x7fffffu) > 0x700000u ? 1 : 0), -127);
+            const float inv = __uint_as_float((uint32_t)(127 - s) << 23), scale = mx_scale_f32((uint32_t)(s + 127));
             uint32_t bits = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (bad) { x[e] = 0.f; continue; }
-                const float a = ldexpf(fabsf(x[e]), -s);
+                const float a = fabsf(x[e]) * inv;
                 // codes count steps of 1/8 below 2, 1/4 below 4, 1/2 up to 7.5
-                const int c = a < 2.f ? (int)rintf(a * 8.f) : a < 4.f ? (int)rintf(a * 4.f) + 8 : min((int)rintf(a * 2.f) + 16, 31);
-                const float v = c < 16 ? c * 0.125f : c < 24 ? (c - 8) * 0.25f : (c - 16) * 0.5f;
-                const uint32_t neg = __float_as_uint(x[e]) >> 31;
-                bits |= ((uint32_t)c | neg << 5) << (6 * e);
-                x[e] -= ldexpf(neg ? -v : v, s);                        // exact: both are multiples of x's last place
+                const float per = a < 2.f ? 8.f : a < 4.f ? 4.f : 2.f, step = a < 2.f ? 0.125f : a < 4.f ? 0.25f : 0.5f;
+                const float c = rintf(a * per), v = c * step;
+                const uint32_t neg = __float_as_uint(x[e]) >> 31, code = (uint32_t)((int)c + (a < 2.f ? 0 : a < 4.f ? 8 : 16));
+                bits |= (code | neg << 5) << (6 * e);
+                x[e] -= (neg ? -v : v) * scale;                         // exact: both are multiples of x's last place
             }
             uint8_t* part = block + ((size_t)quad * parts + p) * part_bytes;
             // the lane's 24 bits are bytes 3 sub .. 3 sub + 2 of the block's 24
@@ -367,6 +386,10 @@ mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, 
     if (tid == 0 && q < nq) {
         info[q] = {red[0] + red[1] + red[2] + red[3] + least, red[4] + red[5] + red[6] + red[7] + least};
         if (todo) todo[q] = 0;
+        if (tau) {
+            tau[q] = -FLT_MAX;
+            row_below[q] = 0;
+        }
     }
 }
 
@@ -404,19 +427,19 @@ struct MxParams {
     int64_t N;                   // rows of the index
     int nq, d, nks, nkq;
     int S;                       // splits: workgroups that share a query block
-    int64_t g0, gstep;           // wave tile t covers the MX_RG groups from g0 + t * gstep
+    int64_t g0, gstep;           // wave tile t covers the RG groups from g0 + t * gstep
     int64_t ntiles;
     // scores
     float* out;                  // [nq][ld]
-    int64_t ld, row0, n;         // columns 0 .. n - 1 are rows row0 ..; row0 < 0: column = MX_TILE t + row of the tile
+    int64_t ld, row0, n;         // columns 0 .. n - 1 are rows row0 ..; row0 < 0: column = 32 RG t + row of the tile
     const void* q;               // the caller's queries (recomputation of those with NaN / inf elements), or null
     int q_dtype;
     const MxQueryInfo* info;
     // search
     const float* tau;            // [nq] floor: a hit scores above it, or equals it with row < row_below
     const uint32_t* row_below;   // [nq] a multiple of 32
-    uint64_t* cand;              // [nq][S][cap] keys of the hits
-    int* cnt;                    // [nq][S]
+    uint2* cand;                 // [nq][S * waves * 2][cap] hits: row, score bits
+    int* cnt;                    // [nq][S * waves * 2]
     int* todo;                   // [nq] set to 1 when a list overflows
     int cap;
 };
@@ -445,23 +468,23 @@ __device__ __forceinline__ void static_for(F&& f) {
     }
 }
 
-// One wave: 128 rows (RG = 4 groups) x BQ = 32 CG queries; 8 waves a workgroup, which share the query block in LDS and
+// One wave: 32 RG rows x BQ = 32 CG queries; WAVES waves a workgroup, which share the query block in LDS and
 // nothing else: while the whole block fits (RESIDENT) the main loop has no barrier. The loop steps through quads of K-sets
 // (256 elements), the quads of a tile and on to the next tile. A K-set's row operands wait in registers: the slot of a
-// K-set is loaded again, for the next quad, as soon as its last MFMA is issued, so four K-sets are in flight (16 KiB a wave,
-// 128 KiB a CU). The query operands of the next part are read from LDS while the current part is multiplied: RG x CG MFMAs
+// K-set is loaded again, for the next quad, as soon as its last MFMA is issued, so four K-sets are in flight (RG = 4: 16 KiB
+// a wave). The query operands of the next part are read from LDS while the current part is multiplied: RG x CG MFMAs
 // per CG reads of 24 bytes a lane.
 // Tiles are dealt round-robin over a query block's S workgroups, then over their waves. When the query block does not fit (long
 // vectors), its quads go through LDS one at a time, all waves in step.
 // MX_SCORES: queries are the A operand, so that a lane holds one row and a store instruction writes two lines of 32
 // consecutive columns (with rows as A: 32 pieces of 32 bytes, one query each; 8192 x 32768 scores took 500 us so).
 // MX_SEARCH: rows are the A operand: a lane holds 16 rows of one query and its floor.
-template <int CG, int PARTS, int FMT, int MODE, bool RESIDENT>
-__global__ void __launch_bounds__(MX_THREADS)
+template <int CG, int RG, int WAVES, int PARTS, int FMT, int MODE, bool RESIDENT>
+__global__ void __launch_bounds__(WAVES * 64)
 mx4_product_kernel(const MxParams p) {
-    constexpr int RG = MX_RG, BQ = 32 * CG, PART = mx_part_bytes<FMT>(BQ), QUAD = PARTS * PART, CODES = mx_code_bytes<FMT>();
+    constexpr int BQ = 32 * CG, PART = mx_part_bytes<FMT>(BQ), QUAD = PARTS * PART, CODES = mx_code_bytes<FMT>();
+    constexpr int TILE = RG * MX_GROUP, THREADS = WAVES * 64;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int* cnts = (int*)(smem + (size_t)(RESIDENT ? p.nkq : 1) * QUAD);   // [BQ]  (MX_SEARCH)
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nqb = (int)gridDim.x / p.S;
@@ -471,8 +494,13 @@ mx4_product_kernel(const MxParams p) {
     const int split = logical / nqb, qb = logical - split * nqb;
     const char* qblock = (const char*)p.Q + (size_t)qb * p.nkq * QUAD;
 
+    // MX_SEARCH: per 32 queries, the lane's floor and its own list of hits (its half of the wave's rows, one query): nobody
+    // else appends to it, so a hit costs a store and an addition
     float tau[CG];
-    uint32_t below[CG];
+    uint32_t below[CG], at[CG];         // at: byte offset of the next hit behind the query block's lists
+    const uint32_t list_bytes = (uint32_t)p.cap * 8, nlists = (uint32_t)p.S * WAVES * 2;
+    char* const lists = (char*)p.cand + (size_t)qb * BQ * nlists * list_bytes;
+    auto list_start = [&](int c) { return ((uint32_t)(c * 32 + l31) * nlists + (split * WAVES + wave) * 2 + h) * list_bytes; };
     int redo = 0;                       // MX_SCORES: a query of this block is not finite
     if constexpr (MODE == MX_SEARCH) {
 #pragma unroll
@@ -480,8 +508,8 @@ mx4_product_kernel(const MxParams p) {
             const int q = qb * BQ + c * 32 + l31;
             tau[c] = q < p.nq ? p.tau[q] : INFINITY;
             below[c] = q < p.nq ? p.row_below[q] : 0;
+            at[c] = list_start(c);
         }
-        for (int i = tid; i < BQ; i += MX_THREADS) cnts[i] = 0;
     } else if (p.q) {
 #pragma unroll
         for (int c = 0; c < CG; ++c) {
@@ -492,12 +520,12 @@ mx4_product_kernel(const MxParams p) {
     auto stage = [&](int quad0, int quads) {
         const uint4* s = (const uint4*)(qblock + (size_t)quad0 * QUAD);
 #pragma unroll 4
-        for (int i = tid; i < quads * (QUAD / 16); i += MX_THREADS) ((uint4*)smem)[i] = s[i];
+        for (int i = tid; i < quads * (QUAD / 16); i += THREADS) ((uint4*)smem)[i] = s[i];
     };
     if constexpr (RESIDENT) stage(0, p.nkq);
     __syncthreads();
 
-    const int64_t per_round = (int64_t)p.S * 8;
+    const int64_t per_round = (int64_t)p.S * WAVES;
     const int64_t rounds = (p.ntiles + per_round - 1) / per_round;
     const int64_t tile0 = (int64_t)wave * p.S + split;
     const size_t group_bytes = (size_t)p.nks * MX_SET_BYTES, group_scales = (size_t)p.nkq * 256;
@@ -508,10 +536,10 @@ mx4_product_kernel(const MxParams p) {
     uint32_t xs[RG], xs_next[RG];
     auto group_of = [&](int64_t tile) { return p.g0 + (tile < p.ntiles ? tile : p.ntiles - 1) * p.gstep; };
     // (buffer loads: the tile's address in scalar registers, the lane's part a 32-bit offset)
-    const int set_bytes = (int)group_bytes, scale_bytes = (int)group_scales;
+    const int alone_ks = p.nks & 1 ? p.nks - 1 : -1, set_bytes = (int)group_bytes, scale_bytes = (int)group_scales;
     auto load_slot = [&](uint4 (&a)[RG], const __amdgpu_buffer_rsrc_t x, int ks) {
         ks = ks < p.nks ? ks : p.nks - 1;                              // (behind the last K-set: loaded, not multiplied)
-        const bool alone = (ks & 1) == 0 && ks + 1 == p.nks;
+        const bool alone = ks == alone_ks;
         const int at = (ks >> 1) * 2 * MX_SET_BYTES + (ks & 1) * 32;
 #pragma unroll
         for (int r = 0; r < RG; ++r)
@@ -527,7 +555,9 @@ mx4_product_kernel(const MxParams p) {
 
     // ---- query operands: 32 queries of one part and K-set at a time
     struct Part { uint4 lo; uint2 hi; };
-    Part B[2];
+    constexpr int NB = RG >= 4 ? 2 : 4;      // reads in flight: NB - 1 steps of RG MFMAs
+    constexpr int STEPS = 4 * PARTS * CG;
+    Part B[NB];
     uint32_t qs[PARTS][CG], qs_first[CG];
     const uint32_t q16 = (h * BQ + l31) * 16, q8 = (h * BQ + l31) * 8, q4 = (h * BQ + l31) * 4;
     auto load_part = [&](Part& b, const char* quad_lds, int j, int part, int c) {
@@ -541,31 +571,30 @@ mx4_product_kernel(const MxParams p) {
     };
 
     f32x16 acc[RG][CG];
-    auto clear = [&]() {
-#pragma unroll
-        for (int r = 0; r < RG; ++r)
-#pragma unroll
-            for (int c = 0; c < CG; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[r][c][i] = 0.f;
-    };
-
     auto finish = [&](int64_t tile) {
         const int64_t g = p.g0 + tile * p.gstep;
         if constexpr (MODE == MX_SCORES) {
 #pragma unroll
             for (int r = 0; r < RG; ++r) {
-                const int64_t col = (p.row0 < 0 ? tile * MX_TILE + r * 32 : (g + r) * 32 - p.row0) + l31;
+                const int64_t col = (p.row0 < 0 ? tile * TILE + r * 32 : (g + r) * 32 - p.row0) + l31;
                 if (col < 0 || col >= p.n) continue;
+                // (a row of the output at a time in scalar registers, the lane's column and its half of the rows as an offset)
+                const uint32_t at0 = (uint32_t)(4 * h * p.ld + col) * 4;
+                const char* o = (const char*)p.out + (size_t)qb * BQ * p.ld * 4;
+                if ((qb + 1) * BQ <= p.nq) {
 #pragma unroll
-                for (int c = 0; c < CG; ++c) {
-                    const int q0 = qb * BQ + c * 32 + 4 * h;
-                    float* o = p.out + (size_t)q0 * p.ld + col;
+                    for (int c = 0; c < CG; ++c)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int at = (i & 3) + 8 * (i >> 2);
-                        if (q0 + at < p.nq) o[(size_t)at * p.ld] = acc[r][c][i];
-                    }
+                        for (int i = 0; i < 16; ++i)
+                            *(float*)(o + (size_t)(c * 32 + (i & 3) + 8 * (i >> 2)) * p.ld * 4 + at0) = acc[r][c][i];
+                } else {
+#pragma unroll
+                    for (int c = 0; c < CG; ++c)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int at = c * 32 + (i & 3) + 8 * (i >> 2);
+                            if (qb * BQ + at + 4 * h < p.nq) *(float*)(o + (size_t)at * p.ld * 4 + at0) = acc[r][c][i];
+                        }
                 }
                 if (redo)
 #pragma unroll 1
@@ -576,45 +605,29 @@ mx4_product_kernel(const MxParams p) {
                     }
             }
         } else {
-            // Hits of a lane: 16 rows of one query in each of the RG groups, as a bit mask per group; then one LDS atomic
-            // per lane and 32 queries takes room for all of them (an atomic per hit, each waited for, cost more than the
-            // products at 1000 hits of 500k rows). row_below is a multiple of 32: a group lies on one side of it.
+            // (row_below is a multiple of 32: a group lies on one side of it)
 #pragma unroll
             for (int c = 0; c < CG; ++c) {
-                uint32_t mask[RG];
-                int n = 0;
+                const uint32_t end = list_start(c) + list_bytes;
 #pragma unroll
                 for (int r = 0; r < RG; ++r) {
                     const uint32_t doc0 = (uint32_t)(g + r) * 32;
+                    if (doc0 + 32 > (uint32_t)p.N)                                         // rows behind the last one
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (doc0 + 4 * h + (i & 3) + 8 * (i >> 2) >= (uint32_t)p.N) acc[r][c][i] = -INFINITY;
+                    const float floor = doc0 < below[c] ? f32_below(tau[c]) : tau[c];      // hits score above it
                     float m = acc[r][c][0];
 #pragma unroll
                     for (int i = 1; i < 16; ++i) m = fmaxf(m, acc[r][c][i]);
-                    const float floor = doc0 < below[c] ? f32_below(tau[c]) : tau[c];      // hits score above it
-                    mask[r] = 0;
-                    if (__any(m > floor)) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) mask[r] |= acc[r][c][i] > floor ? 1u << i : 0u;
-                        if (doc0 + 32 > (uint32_t)p.N)                                     // rows behind the last one
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (doc0 + 4 * h + (i & 3) + 8 * (i >> 2) >= (uint32_t)p.N) mask[r] &= ~(1u << i);
-                        n += __popc(mask[r]);
-                    }
-                }
-                if (!__any(n)) continue;
-                // (the empty asm keeps the compiler from holding these in registers through the main loop)
-                uint32_t ql = c * 32 + l31, h4 = 4 * h;
-                asm volatile("" : "+v"(ql), "+v"(h4));
-                int pos = n ? atomicAdd(&cnts[ql], n) : 0;
-                uint64_t* list = p.cand + ((size_t)(qb * BQ + ql) * p.S + split) * p.cap;
-#pragma unroll
-                for (int r = 0; r < RG; ++r) {
-                    if (!__any(mask[r])) continue;
+                    if (!__any(m > floor)) continue;
+                    uint32_t row = doc0 + 4 * h;
+                    asm volatile("" : "+v"(row));      // (keeps 16 sums of it out of registers in the main loop)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (mask[r] >> i & 1) {
-                            if (pos < p.cap) list[pos] = make_key(acc[r][c][i], (uint32_t)(g + r) * 32 + h4 + (i & 3) + 8 * (i >> 2));
-                            ++pos;
+                        if (acc[r][c][i] > floor) {
+                            if (at[c] < end) *(uint2*)(lists + at[c]) = make_uint2(row + (i & 3) + 8 * (i >> 2), __float_as_uint(acc[r][c][i]));
+                            at[c] += 8;
                         }
                 }
             }
@@ -632,10 +645,9 @@ mx4_product_kernel(const MxParams p) {
             load_scales(xs, scales_of(g), 0);
         }
         if constexpr (RESIDENT) {
-            load_part(B[0], smem, 0, 0, 0);
+            static_for<0, NB - 1>([&](auto u) { load_part(B[u], smem, u / (PARTS * CG), u / CG % PARTS, u % CG); });
             load_part_scales(qs_first, smem, 0);
         }
-        clear();
         while (true) {
             const bool last = quad + 1 == p.nkq;
             const int nquad = last ? 0 : quad + 1;
@@ -647,25 +659,22 @@ mx4_product_kernel(const MxParams p) {
                 __syncthreads();
                 stage(quad, 1);
                 __syncthreads();
-                load_part(B[0], here, 0, 0, 0);
+                static_for<0, NB - 1>([&](auto u) { load_part(B[u], here, u / (PARTS * CG), u / CG % PARTS, u % CG); });
                 load_part_scales(qs_first, here, 0);
             }
             const __amdgpu_buffer_rsrc_t next = codes_of(ng);
             load_scales(xs_next, scales_of(ng), nquad);
 #pragma unroll
             for (int c = 0; c < CG; ++c) qs[0][c] = qs_first[c];
-            static_for<0, 4 * PARTS * CG>([&](auto tc) {
+            static_for<0, STEPS>([&](auto tc) {
                 constexpr int T = decltype(tc)::value, j = T / (PARTS * CG), part = T / CG % PARTS, c = T % CG;
-                constexpr int U = T + 1, jn = U / (PARTS * CG), pn = U / CG % PARTS, cn = U % CG;
-                const Part& b = B[T & 1];
-                Part& bn = B[U & 1];
-                if constexpr (jn < 4) {
-                    load_part(bn, here, jn, pn, cn);
-                    if constexpr (jn == 0 && cn == 0) load_part_scales(qs[pn], here, pn);
-                } else if constexpr (RESIDENT) {
-                    load_part(bn, there, 0, 0, 0);
-                    load_part_scales(qs_first, there, 0);
-                }
+                constexpr int U = T + NB - 1, jn = U / (PARTS * CG), pn = U / CG % PARTS, cn = U % CG;
+                static_assert(STEPS % NB == 0 && NB <= STEPS, "the ring's places are the same in every quad");
+                const Part& b = B[T % NB];
+                if constexpr (U < STEPS) load_part(B[U % NB], here, jn, pn, cn);
+                else if constexpr (RESIDENT) load_part(B[U % NB], there, (U - STEPS) / (PARTS * CG), (U - STEPS) / CG % PARTS, (U - STEPS) % CG);
+                if constexpr (T + 1 < STEPS && (T + 1) / (PARTS * CG) == 0 && (T + 1) % CG == 0) load_part_scales(qs[(T + 1) / CG % PARTS], here, (T + 1) / CG % PARTS);
+                if constexpr (T + 1 == STEPS && RESIDENT) load_part_scales(qs_first, there, 0);
                 __builtin_amdgcn_sched_barrier(0);
                 if (quad * 4 + j < p.nks) {
                     i32x8 qv = {(int)b.lo.x, (int)b.lo.y, (int)b.lo.z, (int)b.lo.w, 0, 0, 0, 0};
@@ -673,13 +682,19 @@ mx4_product_kernel(const MxParams p) {
                         qv[4] = (int)b.hi.x;
                         qv[5] = (int)b.hi.y;
                     }
-#pragma unroll
-                    for (int r = 0; r < RG; ++r) {
+                    auto times = [&](int r, const f32x16& sum) {
                         const i32x8 xv = {(int)A[j][r].x, (int)A[j][r].y, (int)A[j][r].z, (int)A[j][r].w, 0, 0, 0, 0};
                         if constexpr (MODE == MX_SCORES)
-                            acc[r][c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qv, xv, acc[r][c], FMT, MX_E2M1, j, (int)qs[part][c], j, (int)xs[r]);
+                            return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qv, xv, sum, FMT, MX_E2M1, j, (int)qs[part][c], j, (int)xs[r]);
                         else
-                            acc[r][c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xv, qv, acc[r][c], MX_E2M1, FMT, j, (int)xs[r], j, (int)qs[part][c]);
+                            return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xv, qv, sum, MX_E2M1, FMT, j, (int)xs[r], j, (int)qs[part][c]);
+                    };
+                    if (j == 0 && part == 0 && quad == 0) {            // a tile's first products: on top of nothing
+#pragma unroll
+                        for (int r = 0; r < RG; ++r) acc[r][c] = times(r, f32x16{});
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < RG; ++r) acc[r][c] = times(r, acc[r][c]);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -689,7 +704,6 @@ mx4_product_kernel(const MxParams p) {
             for (int r = 0; r < RG; ++r) xs[r] = xs_next[r];
             if (last) {
                 if (tile < p.ntiles) finish(tile);
-                clear();
                 if (++round == rounds || (RESIDENT && ntile >= p.ntiles)) break;
             }
             tile = ntile;
@@ -698,13 +712,13 @@ mx4_product_kernel(const MxParams p) {
     }
 
     if constexpr (MODE == MX_SEARCH) {
-        __syncthreads();
-        for (int i = tid; i < BQ; i += MX_THREADS) {
-            const int q = qb * BQ + i;
+#pragma unroll
+        for (int c = 0; c < CG; ++c) {
+            const int q = qb * BQ + c * 32 + l31;
             if (q >= p.nq) continue;
-            const int n = cnts[i];
-            p.cnt[(size_t)q * p.S + split] = n < p.cap ? n : p.cap;
-            if (n > p.cap) p.todo[q] = 1;
+            const uint32_t n = (at[c] - list_start(c)) / 8;
+            p.cnt[(size_t)q * nlists + (split * WAVES + wave) * 2 + h] = (int)min(n, (uint32_t)p.cap);
+            if (n > (uint32_t)p.cap) p.todo[q] = 1;
         }
     }
 }
@@ -835,60 +849,60 @@ mx4_floor_kernel(const float* __restrict__ sample, int j, int64_t N, float* __re
 }
 
 // ---- the hits of one query -> its best kc, sorted --------------------------------------------------------------
-// lists: [nq][S][cap] keys in any order, cnt[q * S + s] of them. One workgroup of 1024 per query. Few more hits than wanted
-// is the rule (mx4_floor_kernel): a histogram of the scores between the lowest and the best hit, linear in the bits, finds
-// the step that holds the kc-th; everything from that step up (a few more than kc) is sorted in LDS (Pmax slots). Should
-// that be more than the slots (equal scores), the kc-th key is found exactly, 8 bits a pass.
+// lists: [nq][nlists][cap] hits in any order, cnt[q * nlists + l] of them. One workgroup of 1024 per query, nlists <= 8192.
+// Little more hits than wanted is the rule (mx4_floor_kernel). A histogram of the scores between the lowest and the best
+// hit, linear in the bits, finds the step that holds the kc-th; the hits from that step up go to their step's place in LDS
+// (Pmax slots), where each counts the better ones of its own step: its place in the list, no sort. Should they be more than
+// the slots (equal scores), the kc-th key is found exactly, 8 bits a pass, and the kc best are one step.
 constexpr int MX_HELD = 4096;            // hits that are kept in LDS between the passes
 __global__ void __launch_bounds__(1024)
-mx4_select_kernel(const uint64_t* __restrict__ lists, const int* __restrict__ cnt, int S, int cap, int kc, int Pmax, int64_t id_base,
+mx4_select_kernel(const uint2* __restrict__ lists, const int* __restrict__ cnt, int nlists, int cap, int kc, int Pmax, int64_t id_base,
                   float* __restrict__ outD, int64_t* __restrict__ outI) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    uint64_t* sorted = (uint64_t*)smem;                        // [Pmax]
-    uint64_t* held = sorted + Pmax;                            // [MX_HELD]
-    int* off = (int*)(held + MX_HELD);                         // [S]
-    __shared__ int hist[2048];
+    uint64_t* placed = (uint64_t*)smem;                        // [Pmax]
+    uint64_t* held = placed + Pmax;                            // [MX_HELD]
+    __shared__ int hist[2048], fill[2048];                     // hits of a step, then the place of its first; hits placed
     __shared__ uint32_t s_lo[16], s_hi[16];
-    __shared__ int s_sum[16], s_total, s_bin, s_n, s_need;
+    __shared__ int s_sum[16], s_m, s_bin, s_n, s_need;
     __shared__ uint64_t s_prefix;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t q = blockIdx.x;
-    const uint64_t* base = lists + (size_t)q * S * cap;
-    // the lists' places in `held`: S <= 1024
-    const int mine = tid < S ? cnt[q * S + tid] : 0;
-    int run = mine;
+    const uint2* base = lists + (size_t)q * nlists * cap;
+    auto block_scan = [&](int x) {                             // inclusive; one __syncthreads before the next call
+        int run = x;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(run, o); if (lane >= o) run += x; }
-    if (lane == 63) s_sum[wave] = run;
-    hist[tid] = 0;
-    hist[tid + 1024] = 0;
+        for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(run, o); if (lane >= o) run += y; }
+        if (lane == 63) s_sum[wave] = run;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) run += s_sum[w];
+        return run;
+    };
+    for (int i = tid; i < 2048; i += 1024) { hist[i] = 0; fill[i] = 0; }
+    if (tid == 0) { s_n = 0; s_bin = 0; }
     __syncthreads();
-    for (int w = 0; w < wave; ++w) run += s_sum[w];
-    if (tid < S) off[tid] = run - mine;
-    if (tid == 1023) s_total = run;
-    if (tid == 0) { s_bin = 0; s_n = 0; }
-    __syncthreads();
-    const int T = s_total;
-    const bool keep = T <= MX_HELD;
-    // 2^g lanes to a list
+    // 2^g lanes to a list; a list's hits take their places in `held` as they come
     int g = 0;
-    while ((S << (g + 1)) <= 1024) ++g;
-    auto each_key = [&](auto&& f) {
-        for (int s = tid >> g; s < S; s += 1024 >> g) {
-            const int n = (s + 1 < S ? off[s + 1] : T) - off[s];
-            for (int e = tid & ((1 << g) - 1); e < n; e += 1 << g) f(base[(size_t)s * cap + e], off[s] + e);
+    while ((nlists << (g + 1)) <= 1024) ++g;
+    auto each_listed = [&](auto&& f) {
+        for (int l = tid >> g; l < nlists; l += 1024 >> g) {
+            const int n = cnt[q * nlists + l];
+            for (int e = tid & ((1 << g) - 1); e < n; e += 1 << g) {
+                const uint2 hit = base[(size_t)l * cap + e];
+                f(make_key(__uint_as_float(hit.y), hit.x));
+            }
         }
     };
-    auto each_held = [&](auto&& f) {
-        if (keep) for (int e = tid; e < T; e += 1024) f(held[e]);
-        else each_key([&](uint64_t key, int) { f(key); });
-    };
     uint32_t lo = 0xffffffffu, hi = 0;
-    each_key([&](uint64_t key, int at) {
+    each_listed([&](uint64_t key) {
         const uint32_t v = (uint32_t)(key >> 32);
         lo = min(lo, v);
         hi = max(hi, v);
-        if (keep) held[at] = key;
+        const uint64_t here = __ballot(1);                     // one atomic for the lanes that are here
+        const int before = (int)__popcll(here & ((1ull << lane) - 1));
+        int at = 0;
+        if (before == 0) at = atomicAdd(&s_n, (int)__popcll(here));
+        at = __shfl(at, __ffsll((unsigned long long)here) - 1) + before;
+        if (at < MX_HELD) held[at] = key;
     });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -899,45 +913,43 @@ mx4_select_kernel(const uint64_t* __restrict__ lists, const int* __restrict__ cn
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 16; ++w) { lo = min(lo, s_lo[w]); hi = max(hi, s_hi[w]); }
-    int shift = 0;
-    if (T > kc) {
-        while (((hi - lo) >> shift) >= 2048) ++shift;
-        each_held([&](uint64_t key) { atomicAdd(&hist[(hi - (uint32_t)(key >> 32)) >> shift], 1); });
-        __syncthreads();
+    const int T = s_n;
+    auto each = [&](auto&& f) {
+        if (T <= MX_HELD) for (int e = tid; e < T; e += 1024) f(held[e]);
+        else each_listed(f);
+    };
+    int shift = T > 0 ? max(0, 21 - __clz((int)((hi - lo) | 1u))) : 0;      // (hi - lo) >> shift < 2048
+    auto step_of = [&](uint64_t key) { return (int)((hi - (uint32_t)(key >> 32)) >> shift); };
+    each([&](uint64_t key) { atomicAdd(&hist[step_of(key)], 1); });
+    __syncthreads();
+    {
         const int c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
-        int acc = c0 + c1;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(acc, o); if (lane >= o) acc += x; }
-        if (lane == 63) s_sum[wave] = acc;
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) acc += s_sum[w];
-        const int before = acc - c0 - c1;
-        if (before < kc && acc >= kc) {
+        const int run = block_scan(c0 + c1), before = run - c0 - c1;
+        if (before < kc && run >= kc) {
             const bool second = before + c0 < kc;
             s_bin = 2 * tid + (second ? 1 : 0);
-            s_n = second ? acc : before + c0;
+            s_m = second ? run : before + c0;
         }
-        __syncthreads();
+        if (tid == 1023 && run < kc) { s_bin = 2047; s_m = run; }
+        hist[2 * tid] = before;
+        hist[2 * tid + 1] = before + c0;
     }
-    const bool few = T <= kc || s_n <= Pmax;
-    const uint32_t bin = (uint32_t)s_bin;
     __syncthreads();
-    int m;
-    if (few) {
-        if (tid == 0) s_n = 0;
-        __syncthreads();
-        each_held([&](uint64_t key) {
-            if (T <= kc || (hi - (uint32_t)(key >> 32)) >> shift <= bin) sorted[atomicAdd(&s_n, 1)] = key;
+    const int last = s_bin;
+    int m = s_m;                                               // hits in steps up to `last`
+    if (m <= Pmax) {
+        each([&](uint64_t key) {
+            const int b = step_of(key);
+            if (b <= last) placed[hist[b] + atomicAdd(&fill[b], 1)] = key;
         });
-        __syncthreads();
-        m = s_n;
     } else {
         if (tid == 0) { s_prefix = 0; s_need = kc; s_n = 0; }
         for (int sh = 56; sh >= 0; sh -= 8) {
+            __syncthreads();
             if (tid < 256) hist[tid] = 0;
             __syncthreads();
             const uint64_t prefix = s_prefix;
-            each_held([&](uint64_t key) {
+            each([&](uint64_t key) {
                 if (sh == 56 || (key >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[(int)(key >> sh) & 255], 1);
             });
             __syncthreads();
@@ -947,39 +959,29 @@ mx4_select_kernel(const uint64_t* __restrict__ lists, const int* __restrict__ cn
                 s_need -= acc;
                 s_prefix = prefix | (uint64_t)b << sh;
             }
-            __syncthreads();
         }
-        const uint64_t kth = s_prefix;                         // keys are distinct: kc of them reach it
-        each_held([&](uint64_t key) { if (key >= kth) { const int at = atomicAdd(&s_n, 1); if (at < Pmax) sorted[at] = key; } });
         __syncthreads();
+        const uint64_t kth = s_prefix;                         // keys are distinct: kc of them reach it
+        each([&](uint64_t key) { if (key >= kth) { const int at = atomicAdd(&s_n, 1); if (at < Pmax) placed[at] = key; } });
         m = kc;
+        shift = 32;                                            // one step
+        if (tid == 0) { hist[0] = 0; fill[0] = kc; }
     }
-    int P = 2;
-    while (P < m) P <<= 1;
-    for (int i = m + tid; i < P; i += 1024) sorted[i] = 0ull;
     __syncthreads();
-    for (int size = 2; size <= P; size <<= 1)
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            for (int i = tid; i < (P >> 1); i += 1024) {
-                const int a = ((i & ~(stride - 1)) << 1) | (i & (stride - 1)), b = a + stride;
-                const bool desc = (a & size) == 0;
-                const uint64_t x = sorted[a], y = sorted[b];
-                if ((x < y) == desc) { sorted[a] = y; sorted[b] = x; }
-            }
-            __syncthreads();
+    for (int i = tid; i < m; i += 1024) {
+        const uint64_t key = placed[i];
+        const int b = shift == 32 ? 0 : step_of(key), from = hist[b], to = from + fill[b];
+        int at = from;
+        for (int x = from; x < to; ++x) at += placed[x] > key ? 1 : 0;
+        if (at < kc) {
+            outD[q * kc + at] = f32_unordered((uint32_t)(key >> 32));
+            outI[q * kc + at] = id_base + (int64_t)(uint32_t)(~(uint32_t)key);
         }
-    for (int i = tid; i < kc; i += 1024) {
-        const uint64_t key = i < m ? sorted[i] : 0ull;
-        outD[q * kc + i] = key ? f32_unordered((uint32_t)(key >> 32)) : -FLT_MAX;
-        outI[q * kc + i] = key ? id_base + (int64_t)(uint32_t)(~(uint32_t)key) : -1;
     }
-}
-
-// an index that is searched without a sample: every row that is a number is a hit
-__global__ void __launch_bounds__(256)
-mx4_no_floor_kernel(int nq, float* __restrict__ tau, uint32_t* __restrict__ row_below) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < nq) { tau[i] = -FLT_MAX; row_below[i] = 0; }
+    for (int i = m + tid; i < kc; i += 1024) {
+        outD[q * kc + i] = -FLT_MAX;
+        outI[q * kc + i] = -1;
+    }
 }
 
 }  // namespace ipx

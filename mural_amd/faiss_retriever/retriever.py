@@ -126,8 +126,7 @@ class FlatIPIndex:
             I = torch.empty((n, k), dtype=torch.int64, device=x.device)
         else:
             D, I = out
-        _lib.check(L.ipx_search(self._h, C.c_void_p(x.data_ptr()), n, k, C.c_void_p(D.data_ptr()),
-                                C.c_void_p(I.data_ptr()), 1, _torch_stream(x)))
+        _lib.check(L.ipx_search(self._h, x.data_ptr(), n, k, D.data_ptr(), I.data_ptr(), 1, mx4.stream_of(x.device)))
         return D, I
 
     def search_aspect(self, aspect_emb, weights, k, logits=False):
@@ -170,11 +169,11 @@ class FlatIPIndex:
         L = _lib.lib()
         if _is_torch_tensor(codes):
             codes, scales = mx4.check_torch_pair(codes, scales, self.d, self.device)
-            _lib.check(L.ipx_add_mx4(self._h, C.c_void_p(codes.data_ptr()), C.c_void_p(scales.data_ptr()), codes.shape[0], 1,
-                                     _torch_stream(codes)))
+            _lib.check(L.ipx_add_mx4(self._h, codes.data_ptr(), scales.data_ptr(), codes.shape[0], 1,
+                                     mx4.stream_of(codes.device)))
             return
         codes, scales = mx4.check_numpy_pair(codes, scales, self.d)
-        _lib.check(L.ipx_add_mx4(self._h, C.c_void_p(codes.ctypes.data), C.c_void_p(scales.ctypes.data), codes.shape[0], 0, None))
+        _lib.check(L.ipx_add_mx4(self._h, codes.ctypes.data, scales.ctypes.data, codes.shape[0], 0, None))
 
     def scores(self, q, start=0, n=None):
         """The inner products of every query with rows start .. start + n - 1 (default: all to the end), fp32 [nq, n].
@@ -186,17 +185,17 @@ class FlatIPIndex:
         n = self.ntotal - start if n is None else n
         if _is_torch_tensor(q):
             import torch
-            dt = {torch.float32: _lib.IPX_F32, torch.float16: _lib.IPX_F16, torch.bfloat16: _lib.IPX_BF16}[q.dtype]
+            dt = mx4.torch_types()[q.dtype]
             assert q.is_cuda and q.device.index == self.device
             q = q.contiguous()
             out = torch.empty((nq, max(n, 0)), dtype=torch.float32, device=q.device)
-            _lib.check(L.ipx_scores(self._h, C.c_void_p(q.data_ptr()), dt, nq, start, n, C.c_void_p(out.data_ptr()), 1,
-                                    _torch_stream(q)))
+            _lib.check(L.ipx_scores(self._h, q.data_ptr(), dt, nq, start, n, out.data_ptr(), 1,
+                                    mx4.stream_of(q.device)))
             return out
         q = np.ascontiguousarray(q, dtype=q.dtype if q.dtype in _NP_DTYPES else "float32")
         out = np.empty((nq, max(n, 0)), dtype=np.float32)
-        _lib.check(L.ipx_scores(self._h, C.c_void_p(q.ctypes.data), _NP_DTYPES[q.dtype], nq, start, n,
-                                C.c_void_p(out.ctypes.data), 0, None))
+        _lib.check(L.ipx_scores(self._h, q.ctypes.data, _NP_DTYPES[q.dtype], nq, start, n,
+                                out.ctypes.data, 0, None))
         return out
 
     def scores_mx4(self, codes, scales, start=0, n=None):
@@ -207,13 +206,13 @@ class FlatIPIndex:
             import torch
             codes, scales = mx4.check_torch_pair(codes, scales, self.d, self.device)
             out = torch.empty((codes.shape[0], max(n, 0)), dtype=torch.float32, device=codes.device)
-            _lib.check(L.ipx_scores_mx4(self._h, C.c_void_p(codes.data_ptr()), C.c_void_p(scales.data_ptr()), codes.shape[0],
-                                        start, n, C.c_void_p(out.data_ptr()), 1, _torch_stream(codes)))
+            _lib.check(L.ipx_scores_mx4(self._h, codes.data_ptr(), scales.data_ptr(), codes.shape[0],
+                                        start, n, out.data_ptr(), 1, mx4.stream_of(codes.device)))
             return out
         codes, scales = mx4.check_numpy_pair(codes, scales, self.d)
         out = np.empty((codes.shape[0], max(n, 0)), dtype=np.float32)
-        _lib.check(L.ipx_scores_mx4(self._h, C.c_void_p(codes.ctypes.data), C.c_void_p(scales.ctypes.data), codes.shape[0],
-                                    start, n, C.c_void_p(out.ctypes.data), 0, None))
+        _lib.check(L.ipx_scores_mx4(self._h, codes.ctypes.data, scales.ctypes.data, codes.shape[0],
+                                    start, n, out.ctypes.data, 0, None))
         return out
 
     def lookup(self, ids, scale=None, dtype=None):
@@ -225,16 +224,16 @@ class FlatIPIndex:
         if _is_torch_tensor(ids):
             import torch
             dtype = dtype or torch.float32
-            dt = {torch.float32: _lib.IPX_F32, torch.float16: _lib.IPX_F16, torch.bfloat16: _lib.IPX_BF16}[dtype]
+            dt = mx4.torch_types()[dtype]
             assert ids.dtype == torch.int64 and ids.is_cuda and ids.device.index == self.device
             ids = ids.contiguous()
             if scale is not None:
                 assert scale.shape == ids.shape and scale.device == ids.device
                 scale = scale.contiguous().float()
             out = torch.empty((*ids.shape, self.d), dtype=dtype, device=ids.device)
-            _lib.check(L.ipx_lookup(self._h, C.c_void_p(ids.data_ptr()), ids.numel(),
-                                    None if scale is None else C.c_void_p(scale.data_ptr()), C.c_void_p(out.data_ptr()), dt, 1,
-                                    _torch_stream(ids)))
+            _lib.check(L.ipx_lookup(self._h, ids.data_ptr(), ids.numel(),
+                                    None if scale is None else scale.data_ptr(), out.data_ptr(), dt, 1,
+                                    mx4.stream_of(ids.device)))
             return out
         ids = np.ascontiguousarray(ids, dtype=np.int64)
         if scale is not None:
@@ -242,8 +241,8 @@ class FlatIPIndex:
             assert scale.shape == ids.shape
         dtype = np.dtype(dtype or np.float32)
         out = np.empty((*ids.shape, self.d), dtype=dtype)
-        _lib.check(L.ipx_lookup(self._h, C.c_void_p(ids.ctypes.data), ids.size,
-                                None if scale is None else C.c_void_p(scale.ctypes.data), C.c_void_p(out.ctypes.data),
+        _lib.check(L.ipx_lookup(self._h, ids.ctypes.data, ids.size,
+                                None if scale is None else scale.ctypes.data, out.ctypes.data,
                                 _NP_DTYPES[dtype], 0, None))
         return out
 
