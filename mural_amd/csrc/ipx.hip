@@ -792,11 +792,20 @@ int scan_f32_deep(ipx_index* ix, const float* dq, const float* dw, int A, int lo
 int launch_rescore(const ipx::RescoreParams& rp, int64_t nblocks, hipStream_t st) {
     const int dpad = rp.xfmt == 2 ? (rp.nks + 1) / 2 * 128 : rp.nks * (rp.xfmt ? 32 : 16);
     const int fixed = ((dpad * 4 + 15) & ~15) + rp.P * 8 + (rp.P <= ipx::RS_RANK_SORT || rp.xfmt == 2 ? rp.P * 8 : 0);
-    const int per_wave = rp.xfmt == 2 ? 64 * ipx::RS_ROW : ipx::RS_KB * 16 * ipx::RS_ROW;
+    if (rp.xfmt == 2) {
+        const int per_wave = 64 * ipx::RS_ROW;
+        const bool few = nblocks <= 128 && fixed + 16 * per_wave <= 160 * 1024;
+        const int lds = fixed + (few ? 16 : 4) * per_wave;
+        void (*kern)(const ipx::RescoreParams) = few ? ipx::rescore_kernel<16, true> : ipx::rescore_kernel<4, true>;
+        if (int rc = ensure_dynamic_lds((const void*)kern, lds)) return rc;
+        hipLaunchKernelGGL(kern, dim3((unsigned)nblocks), dim3(few ? 1024 : 256), lds, st, rp);
+        IPX_HIP(hipGetLastError());
+        return 0;
+    }
+    const int per_wave = ipx::RS_KB * 16 * ipx::RS_ROW;
     const int nw = (nblocks <= 128 && fixed + 16 * per_wave <= 160 * 1024) ? 16 : 4;
     const int rlds = fixed + nw * per_wave;
-    void (*kern)(const ipx::RescoreParams) = rp.xfmt == 2 ? (nw == 16 ? ipx::rescore_kernel<16, true> : ipx::rescore_kernel<4, true>)
-                                                          : (nw == 16 ? ipx::rescore_kernel<16> : ipx::rescore_kernel<4>);
+    void (*kern)(const ipx::RescoreParams) = nw == 16 ? ipx::rescore_kernel<16> : ipx::rescore_kernel<4>;
     if (int rc = ensure_dynamic_lds((const void*)kern, rlds)) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)nblocks), dim3(nw * 64), rlds, st, rp);
     IPX_HIP(hipGetLastError());
@@ -1355,12 +1364,25 @@ constexpr int MX_PARTS_SEARCH = 2;       // E2M3 parts per query in the scan: wh
 constexpr int MX_PARTS_SCORES = 5;       // ... in ipx_scores: as exact as fp32
 constexpr int MX_MAX_K = IPX_MAX_K;      // deepest list of a search
 constexpr int MX_SLICE = 4096;           // queries per pass of a search (bounds the workspace)
+constexpr int64_t MX_WHOLE = 4096, MX_WHOLE_PAIRS = 1 << 20;      // scan_mx4_path: rows, rows x queries scored without a scan
 
 // How a product runs: 32-query groups per workgroup, splits of the corpus, whether the query block stays in LDS; the
 // groups of a wave tile and the waves of a workgroup.
-#ifndef MXS_RG
-#define MXS_RG 2
-#define MXS_W 16
+#ifndef MXS_RG1
+#define MXS_RG1 2
+#define MXS_W1 16
+#endif
+#ifndef MXS_RG2
+#define MXS_RG2 2
+#define MXS_W2 8
+#endif
+#ifndef MXF_RG1
+#define MXF_RG1 4
+#define MXF_W1 8
+#endif
+#ifndef MXF_RG2
+#define MXF_RG2 4
+#define MXF_W2 8
 #endif
 struct MxGeom { int cg, rg, waves, nqb, S, lds; bool resident; int64_t ntiles, rounds; };
 MxGeom mx4_geometry(const ipx_index* ix, int64_t nq, int quad_bytes_per_cg, int mode, int64_t groups) {
@@ -1373,8 +1395,8 @@ MxGeom mx4_geometry(const ipx_index* ix, int64_t nq, int quad_bytes_per_cg, int 
     g.resident = g.cg * whole <= room;
     if (!g.resident) g.cg = nq <= 32 ? 1 : 2;
     g.lds = g.resident ? whole * g.cg : quad_bytes_per_cg * g.cg;
-    g.rg = mode == ipx::MX_SEARCH ? 4 : MXS_RG;
-    g.waves = mode == ipx::MX_SEARCH ? 8 : g.cg == 1 ? MXS_W : 8;
+    g.rg = mode == ipx::MX_SEARCH ? (g.cg == 1 ? MXF_RG1 : MXF_RG2) : (g.cg == 1 ? MXS_RG1 : MXS_RG2);
+    g.waves = mode == ipx::MX_SEARCH ? (g.cg == 1 ? MXF_W1 : MXF_W2) : (g.cg == 1 ? MXS_W1 : MXS_W2);
     g.nqb = (int)((nq + 32 * g.cg - 1) / (32 * g.cg));
     g.ntiles = (groups + g.rg - 1) / g.rg;
     // (a short corpus goes to as many CUs as it has tiles: a tile per wave of few workgroups leaves the matrix cores of the
@@ -1388,10 +1410,11 @@ template <int PARTS, int FMT, int MODE>
 int launch_mx4_product(const MxGeom& g, ipx::MxParams p, hipStream_t st) {
     p.S = g.S;
     p.ntiles = g.ntiles;
-    constexpr int RG = MODE == ipx::MX_SEARCH ? 4 : MXS_RG, W1 = MODE == ipx::MX_SEARCH ? 8 : MXS_W, W2 = 8;
+    constexpr bool SEARCH = MODE == ipx::MX_SEARCH;
+    constexpr int R1 = SEARCH ? MXF_RG1 : MXS_RG1, R2 = SEARCH ? MXF_RG2 : MXS_RG2, W1 = SEARCH ? MXF_W1 : MXS_W1, W2 = SEARCH ? MXF_W2 : MXS_W2;
     void (*kern)(const ipx::MxParams) =
-        g.resident ? (g.cg == 1 ? ipx::mx4_product_kernel<1, RG, W1, PARTS, FMT, MODE, true> : ipx::mx4_product_kernel<2, RG, W2, PARTS, FMT, MODE, true>)
-                   : (g.cg == 1 ? ipx::mx4_product_kernel<1, RG, W1, PARTS, FMT, MODE, false> : ipx::mx4_product_kernel<2, RG, W2, PARTS, FMT, MODE, false>);
+        g.resident ? (g.cg == 1 ? ipx::mx4_product_kernel<1, R1, W1, PARTS, FMT, MODE, true> : ipx::mx4_product_kernel<2, R2, W2, PARTS, FMT, MODE, true>)
+                   : (g.cg == 1 ? ipx::mx4_product_kernel<1, R1, W1, PARTS, FMT, MODE, false> : ipx::mx4_product_kernel<2, R2, W2, PARTS, FMT, MODE, false>);
     if (int rc = ensure_dynamic_lds((const void*)kern, std::max(g.lds, 64 * 1024 + 1))) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)(g.nqb * g.S)), dim3(g.waves * 64), g.lds, st, p);
     IPX_HIP(hipGetLastError());
@@ -1454,8 +1477,8 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     int* todo = (int*)((char*)ix->mxq.p + info_bytes + 2 * word);
 
     if (timing) IPX_HIP(hipEventRecord(ix->ev[0], st));
-    hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)(g.nqb * 32 * g.cg)), dim3(256), 0, st, (const void*)qf,
-                       (int)IPX_F32, (int)nq, ix->d, PARTS, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, info, todo,
+    hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)nq), dim3(256), 0, st, (const void*)qf,
+                       (int)IPX_F32, ix->d, PARTS, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, info, todo,
                        direct ? tau : nullptr, below);
     IPX_HIP(hipGetLastError());
     ipx::MxParams p = {};
@@ -1551,6 +1574,38 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
     // The list has to reach e below the k-th score (rescore_kernel, post): 1.8M Gaussian rows of 768, k = 100: 120 left 2 of
     // 64 queries to the repeat pass, 125 none; 500k, k = 1000: 1100 left 131 of 1000, 1150 none. Rows whose norms spread
     // widen e: the list then grows as in the bf16 scan (ipx_index::kc_boost).
+    // A short index and not many queries: the exact score of every row at once, one launch and nothing to prove (and no
+    // synchronisation). 3 queries, 999 rows of 100: 43 us for the passes below. The limit: 16 chains of 64 rows keep a CU busy for about
+    // as long as the passes take.
+    if (ix->ntotal <= MX_WHOLE && nq * ix->ntotal <= MX_WHOLE_PAIRS && ix->force_kc == 0) {
+        if (int rc = ix->mxq.ensure((size_t)nq * sizeof(ipx::MxQueryInfo))) return rc;
+        if (int rc = ix->flags.ensure((size_t)nq * sizeof(int))) return rc;
+        ipx::RescoreParams rp;
+        rp.candD = nullptr;
+        rp.candI = nullptr;
+        rp.q = qf;
+        rp.qmap = nullptr;
+        rescore_rows(ix, rp);
+        rp.qinfo = nullptr;
+        rp.all_rows = (int)ix->ntotal;
+        rp.maxsq = (const uint32_t*)ix->maxsq.p;
+        rp.outD = dD;
+        rp.outI = dI;
+        rp.flags = (int*)ix->flags.p;
+        rp.err = nullptr;
+        rp.outl_count = nullptr;
+        rp.shared_list = 0;
+        rp.nq = (int)nq;
+        rp.id_base = ix->id_base;
+        rp.acc_coef = 1.f;
+        rp.qparts = 1;
+        rp.post = 0;
+        rp.d = ix->d;
+        rp.k = k;
+        rp.kc = 0;
+        rp.P = next_pow2((int)ix->ntotal);
+        return launch_rescore(rp, nq, st);
+    }
     const int kc0 = ix->force_kc > 0 ? ix->force_kc : (int)((int64_t)std::max(128, k + k / 4) * ix->kc_boost / 8);
     const int kc = std::min(std::max(kc0, k), MAX_KC);
     for (int64_t q0 = 0; q0 < nq; q0 += MX_SLICE) {
@@ -1579,8 +1634,7 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
         // (the repeat pass has put other queries' norms where the rescoring kernel reads them)
         if (int rc = ix->Qp.ensure((size_t)((n + 31) / 32) * ix->nkq_x * ipx::mx_part_bytes<ipx::MX_E2M3>(32))) return rc;
         if (int rc = ix->mxq.ensure((size_t)n * sizeof(ipx::MxQueryInfo))) return rc;
-        hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)n), dim3(256), 0, st, (const void*)q, (int)IPX_F32, (int)n,
-                           ix->d, 1, 32, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr,
+        hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)n), dim3(256), 0, st, (const void*)q, (int)IPX_F32, ix->d, 1, 32, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr,
                        (float*)nullptr, (uint32_t*)nullptr);
         IPX_HIP(hipGetLastError());
         if (int rc = exact_rows_path(ix, q, hard, k, D, I, st)) return rc;
@@ -1594,8 +1648,7 @@ int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sca
     ipx::MxParams p = {};
     mx4_rows(ix, p);
     // (a tile is a power of two of groups and the buffers end behind eight: groups up to a tile's end exist)
-    p.g0 = row0 / ipx::MX_GROUP / MXS_RG * MXS_RG;
-    p.gstep = MXS_RG;
+    p.g0 = row0 / ipx::MX_GROUP / 4 * 4;
     const int64_t groups = (row0 + n + ipx::MX_GROUP - 1) / ipx::MX_GROUP - p.g0;
     p.nq = (int)nq;
     p.out = out;
@@ -1605,21 +1658,23 @@ int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sca
     if (q_scales) {
         const int quad1 = ipx::mx_part_bytes<ipx::MX_E2M1>(32);
         const MxGeom g = mx4_geometry(ix, nq, quad1, ipx::MX_SCORES, groups);
+        p.gstep = g.rg;
         if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
-        const int64_t total = (int64_t)g.nqb * 32 * g.cg * ix->nkq_x * 8;
+        const int64_t total = nq * ix->nkq_x * 8;
         hipLaunchKernelGGL(ipx::mx4_pack_codes_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, (const uint8_t*)dq,
-                           q_scales, (int)nq, ix->d, 32 * g.cg, ix->nkq_x, total, (uint8_t*)ix->Qp.p);
+                           q_scales, ix->d, 32 * g.cg, ix->nkq_x, total, (uint8_t*)ix->Qp.p);
         IPX_HIP(hipGetLastError());
         p.Q = (const uint8_t*)ix->Qp.p;
         return launch_mx4_product<1, ipx::MX_E2M1, ipx::MX_SCORES>(g, p, st);
     }
     const int quad1 = MX_PARTS_SCORES * ipx::mx_part_bytes<ipx::MX_E2M3>(32);
     const MxGeom g = mx4_geometry(ix, nq, quad1, ipx::MX_SCORES, groups);
+    p.gstep = g.rg;
     if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
     if (int rc = ix->mxq.ensure((size_t)nq * sizeof(ipx::MxQueryInfo))) return rc;
-    hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)(g.nqb * 32 * g.cg)), dim3(256), 0, st, dq, q_dtype, (int)nq,
-                       ix->d, MX_PARTS_SCORES, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr,
-                       (float*)nullptr, (uint32_t*)nullptr);
+    hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)nq), dim3(256), 0, st, dq, q_dtype, ix->d, MX_PARTS_SCORES,
+                       32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr, (float*)nullptr,
+                       (uint32_t*)nullptr);
     IPX_HIP(hipGetLastError());
     p.Q = (const uint8_t*)ix->Qp.p;
     p.q = dq;

@@ -917,6 +917,7 @@ struct RescoreParams {
     int nkq = 0;
     const float* qinfo = nullptr;         // [nq][2]: |q|^2 and |q - scanned parts|^2 (mx4_pack_queries_kernel)
     const float* floor = nullptr;         // [nq]: the score a candidate had to reach; -FLT_MAX: none
+    int all_rows = 0;                     // > 0: no lists, every query scores rows 0 .. all_rows - 1 of the index
 };
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
@@ -939,6 +940,21 @@ __device__ __forceinline__ int place_in_steps(const uint64_t* keys, int m, uint6
     __shared__ uint32_t s_lo[NW], s_hi[NW];
     __shared__ int s_sum[NW];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (m <= 256) {                             // few keys: every key counts the larger ones at once
+        __syncthreads();
+        if (tid == 0) s_sum[0] = 0;
+        __syncthreads();
+        if (tid < m) {
+            if (const uint64_t key = keys[tid]) {
+                int at = 0;
+                for (int x = 0; x < m; ++x) at += keys[x] > key ? 1 : 0;
+                emit(at, key);
+                atomicAdd(&s_sum[0], 1);
+            }
+        }
+        __syncthreads();
+        return s_sum[0];
+    }
     int *first = steps, *fill = steps + 2048;
     uint32_t lo = 0xffffffffu, hi = 0;
     for (int i = tid; i < m; i += NT) {
@@ -1019,7 +1035,7 @@ rescore_kernel(const RescoreParams p) {
     __syncthreads();
     float qn2 = 0.f, dqn2 = 0.f;
     for (int w = 0; w < NW; ++w) { qn2 += red[w]; dqn2 += red[NW + w]; }
-    if constexpr (MX4) {
+    if (MX4 && p.qinfo) {
         const int64_t qq = p.qmap ? (int64_t)p.qmap[qi] : qi;
         qn2 = p.qinfo[2 * qq];
         dqn2 = p.qinfo[2 * qq + 1];
@@ -1043,7 +1059,8 @@ rescore_kernel(const RescoreParams p) {
     // The list is sorted: valid entries first, scores descending. Its length and the margin cut are counted by all
     // threads at once (one round of loads each) instead of searched by one thread (a dozen dependent loads).
     __shared__ int s_nvalid, s_nge;
-    const bool have_list = !(p.todo && p.todo[qi]);
+    const bool whole = MX4 && p.all_rows > 0;
+    const bool have_list = !whole && !(p.todo && p.todo[qi]);
     if (tid == 0) { s_nvalid = 0; s_nge = 0; }
     __syncthreads();
     // a-priori margin test of a full list: the entries at or above thr = a_k - 2 eps (kc >= k; a list that is not
@@ -1062,7 +1079,9 @@ rescore_kernel(const RescoreParams p) {
     __syncthreads();
     if (tid == 0) {
         int m = 0, flag = 0, post = 0;
-        if (!have_list) {
+        if (whole) {
+            m = p.all_rows;
+        } else if (!have_list) {
             // merge_pool_kernel could not build this query's list (more than its pool of near-ties at the cut):
             // there is no list to rescore; the query is repeated like one whose list failed the margin test
             flag = 1;
@@ -1115,22 +1134,22 @@ rescore_kernel(const RescoreParams p) {
         // mx4 rows: 64 candidates per wave, one per lane — the chain of a candidate is serial, so the lanes are what there is
         // to fill (16 chains a wave took 360 us for 1000 x 1500 candidates of 768). Rows come 64 bytes (128 elements, two
         // K-sets) at a time, one line ahead, four lanes to a line (every lane its own line: each of a line's four loads
-        // misses), and reach their lanes through LDS; a lane fetches its own scales, one quad ahead. Values are exact in
-        // fp32, so the chain is the one a bf16 index of these values runs.
+        // misses), and reach their lanes through LDS; a lane fetches its own scales. Values are exact in fp32, so the chain is
+        // the one a bf16 index of these values runs. (Three lines ahead: 205 instead of 178 us for 1000 x 1250 candidates,
+        // fewer waves fit; 16 instead of 14 for one query.)
         const int nb = (p.d + 31) / 32, nlines = (p.nks + 1) / 2;
-        char* lines = (char*)(sorted + (by_rank ? p.P : 0)) + wave * (64 * RS_ROW);
+        const bool odd = p.nks & 1;
+        char* lines = (char*)(sorted + p.P) + wave * (64 * RS_ROW);
+        auto row_of = [&](int i) { return whole ? (int64_t)(i < m ? i : m - 1) : cI[i < m ? i : m - 1] - p.id_base; };
         for (int g0 = wave * 64; g0 < m; g0 += NT) {
-            const int my = g0 + lane < m ? g0 + lane : m - 1;
-            const int64_t row = cI[my] - p.id_base;
+            const int64_t row = row_of(g0 + lane);
             const uint2* sp = (const uint2*)(p.Xs + (size_t)row * p.nkq * 8);
             // lane 4 r + c fetches piece c of the lines of candidates r, 16 + r, 32 + r, 48 + r
             // (ipx_mx4_kernels.h, mx_code_at: a last K-set without a partner lies in 32-byte pieces; its line is read twice
             // over, the second half is not used)
             // (named registers, not arrays: hipcc keeps an array that is live across the loop in scratch memory)
-            const bool odd = p.nks & 1;
             auto place = [&](int i, int& last) {              // candidate i * 16 + r: its first line; from there to its last
-                const int who = i * 16 + (lane >> 2);
-                const int64_t other = cI[g0 + who < m ? g0 + who : m - 1] - p.id_base;
+                const int64_t other = row_of(g0 + i * 16 + (lane >> 2));
                 const int at = (int)(other & 31) * 64 + (lane & 3) * 16, alone = (int)(other & 31) * 32 + (lane & 1) * 16;
                 last = (nlines - 1) * 2048 + (odd ? alone - at : 0);
                 return (const uint8_t*)p.X + (size_t)(other >> 5) * p.nks * 1024 + at;
@@ -1138,23 +1157,33 @@ rescore_kernel(const RescoreParams p) {
             int e0, e1, e2, e3;
             const uint8_t *x0 = place(0, e0), *x1 = place(1, e1), *x2 = place(2, e2), *x3 = place(3, e3);
             float acc = 0.f;
-            auto fetch = [&](const uint8_t* x, int line, int last) { return *(const uint4*)(x + (line < nlines - 1 ? line * 2048 : last)); };
-            uint4 v0 = fetch(x0, 0, e0), v1 = fetch(x1, 0, e1), v2 = fetch(x2, 0, e2), v3 = fetch(x3, 0, e3);
-            uint2 sc = sp[0];
+            struct Line { uint4 a, b, c, d; uint2 s; };
+            auto fetch = [&](int line) {
+                Line l;
+                const int at = line * 2048;
+                const bool end = line >= nlines - 1;
+                l.a = *(const uint4*)(x0 + (end ? e0 : at));
+                l.b = *(const uint4*)(x1 + (end ? e1 : at));
+                l.c = *(const uint4*)(x2 + (end ? e2 : at));
+                l.d = *(const uint4*)(x3 + (end ? e3 : at));
+                l.s = sp[line / 2 < p.nkq ? line / 2 : p.nkq - 1];
+                return l;
+            };
+            Line next = fetch(0);
             for (int line = 0; line < nlines; ++line) {
                 wave_lds_sync();
                 char* to = lines + (lane >> 2) * RS_ROW + (lane & 3) * 16;
-                *(uint4*)(to) = v0;
-                *(uint4*)(to + 16 * RS_ROW) = v1;
-                *(uint4*)(to + 32 * RS_ROW) = v2;
-                *(uint4*)(to + 48 * RS_ROW) = v3;
-                v0 = fetch(x0, line + 1, e0); v1 = fetch(x1, line + 1, e1); v2 = fetch(x2, line + 1, e2); v3 = fetch(x3, line + 1, e3);
+                *(uint4*)(to) = next.a;
+                *(uint4*)(to + 16 * RS_ROW) = next.b;
+                *(uint4*)(to + 32 * RS_ROW) = next.c;
+                *(uint4*)(to + 48 * RS_ROW) = next.d;
+                const uint2 sc = next.s;
+                next = fetch(line + 1);
                 wave_lds_sync();
                 const uint4* own = (const uint4*)(lines + lane * RS_ROW);
                 const uint4 c[4] = {own[0], own[1], own[2], own[3]};
                 const uint32_t two = (line & 1) * 16;                       // this line's scale bytes of the quad
                 const uint32_t s0 = sc.x >> two, s1 = sc.y >> two;
-                if (line & 1) sc = sp[(line + 1) / 2 < p.nkq ? (line + 1) / 2 : p.nkq - 1];
                 const int blocks = nb - line * 4;                           // 4 except in the last line
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {                               // block b: K-set b >> 1, half b & 1

@@ -319,10 +319,10 @@ struct MxQueryInfo {      // of one query
     float restsq;         // |q - sum of its parts|^2        very small elements vanish, the bounds they stand for must not)
 };
 
-// One workgroup per query (rows beyond nq are written as zeros). Eight lanes per block, four elements each. With `tau`, the
+// One workgroup per query. Eight lanes per block, four elements each. With `tau`, the
 // state of a search without a floor is written too: every row that scores a number is a hit.
 __global__ void __launch_bounds__(256)
-mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, int parts, int bq, int nkq, uint8_t* __restrict__ dst,
+mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int d, int parts, int bq, int nkq, uint8_t* __restrict__ dst,
                         MxQueryInfo* __restrict__ info, int* __restrict__ todo, float* __restrict__ tau, uint32_t* __restrict__ row_below) {
     __shared__ float red[8];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -337,7 +337,7 @@ mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int at = b * 32 + sub * 4 + e;
-            x[e] = q < nq && at < d ? load_as_f32(src, dtype, q * (int64_t)d + at) : 0.f;
+            x[e] = at < d ? load_as_f32(src, dtype, q * (int64_t)d + at) : 0.f;
             ss = fmaf(x[e], x[e], ss);
             nonzero |= x[e] != 0.f;
         }
@@ -383,7 +383,7 @@ mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, 
     for (int off = 32; off > 0; off >>= 1) { ss += __shfl_xor(ss, off); rr += __shfl_xor(rr, off); }
     if (lane == 0) { red[tid >> 6] = ss; red[4 + (tid >> 6)] = rr; }
     const float least = __syncthreads_or(nonzero) ? 1e-37f : 0.f;
-    if (tid == 0 && q < nq) {
+    if (tid == 0) {
         info[q] = {red[0] + red[1] + red[2] + red[3] + least, red[4] + red[5] + red[6] + red[7] + least};
         if (todo) todo[q] = 0;
         if (tau) {
@@ -393,9 +393,9 @@ mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, 
     }
 }
 
-// external mx4 rows as queries (one part, E2M1); one thread per block of every padded query
+// external mx4 rows as queries (one part, E2M1); one thread per block of every query, blocks up to whole quads
 __global__ void __launch_bounds__(256)
-mx4_pack_codes_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int nq, int d, int bq, int nkq,
+mx4_pack_codes_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int d, int bq, int nkq,
                       int64_t total, uint8_t* __restrict__ dst) {
     const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (gid >= total) return;
@@ -403,7 +403,7 @@ mx4_pack_codes_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
     const int b = (int)(gid - q * (nkq * 8)), nb = (d + 31) / 32;
     uint32_t w[4] = {0, 0, 0, 0};
     uint8_t sc = 0;
-    if (q < nq && b < nb) {
+    if (b < nb) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint8_t* s = codes + ((size_t)q * nb + b) * 16 + 4 * i;
@@ -517,6 +517,8 @@ mx4_product_kernel(const MxParams p) {
             redo |= q < p.nq && !(p.info[q].sumsq <= FLT_MAX) ? 1 : 0;
         }
     }
+    // (the packing kernels do not write the places of queries behind the last one: what lies there only reaches sums that are
+    // never stored)
     auto stage = [&](int quad0, int quads) {
         const uint4* s = (const uint4*)(qblock + (size_t)quad0 * QUAD);
 #pragma unroll 4
@@ -698,7 +700,11 @@ mx4_product_kernel(const MxParams p) {
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (part == PARTS - 1 && c == CG - 1) load_slot(A[j], next, nquad * 4 + j);
+                // (the two halves of a 64-byte piece one after the other: the second finds the line in L1)
+                if constexpr (part == PARTS - 1 && c == CG - 1 && (j & 1)) {
+                    load_slot(A[j - 1], next, nquad * 4 + j - 1);
+                    load_slot(A[j], next, nquad * 4 + j);
+                }
             });
 #pragma unroll
             for (int r = 0; r < RG; ++r) xs[r] = xs_next[r];
@@ -883,13 +889,26 @@ mx4_select_kernel(const uint2* __restrict__ lists, const int* __restrict__ cnt, 
     // 2^g lanes to a list; a list's hits take their places in `held` as they come
     int g = 0;
     while ((nlists << (g + 1)) <= 1024) ++g;
+    // (a thread's up to four lists: their lengths and their first hits are on the way together)
     auto each_listed = [&](auto&& f) {
-        for (int l = tid >> g; l < nlists; l += 1024 >> g) {
-            const int n = cnt[q * nlists + l];
-            for (int e = tid & ((1 << g) - 1); e < n; e += 1 << g) {
-                const uint2 hit = base[(size_t)l * cap + e];
-                f(make_key(__uint_as_float(hit.y), hit.x));
+        for (int l0 = tid >> g; l0 < nlists; l0 += 4 * (1024 >> g)) {
+            const int e0 = tid & ((1 << g) - 1);
+            int n[4];
+            uint2 hit[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int l = l0 + u * (1024 >> g);
+                n[u] = l < nlists ? cnt[q * nlists + l] : 0;
             }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (e0 < n[u]) hit[u] = base[(size_t)(l0 + u * (1024 >> g)) * cap + e0];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                for (int e = e0; e < n[u]; e += 1 << g) {
+                    if (e > e0) hit[u] = base[(size_t)(l0 + u * (1024 >> g)) * cap + e];
+                    f(make_key(__uint_as_float(hit[u].y), hit[u].x));
+                }
         }
     };
     uint32_t lo = 0xffffffffu, hi = 0;

@@ -146,6 +146,21 @@ def test_search_equals_the_exact_scores_of_the_stored_values(R, n, d, nq, k, add
     assert_bits(D, I, Q, M.rounded(X), k)
 
 
+@pytest.mark.parametrize("n,d,nq,k", [(1, 8, 3, 4), (33, 1, 2, 7), (777, 768, 1, 100), (257, 16, 256, 128), (4000, 64, 40, 200),
+                                      (4096, 33, 300, 10), (129, 8192, 2, 100)])
+@pytest.mark.parametrize("candidates", [1, 300])
+def test_short_indexes_through_the_scan(R, n, d, nq, k, candidates):
+    """Short indexes are scored row by row; with a list length given they take the scan: the same answer."""
+    X, Q = gaussian(1235, (n, d)), gaussian(4322, (nq, d))
+    X[n // 2] = 0
+    ix = index(R, X)
+    D, I = ix.search(Q, k)
+    assert_bits(D, I, Q, M.rounded(X), k)
+    ix.set_param("bf16_candidates", candidates)
+    D2, I2 = ix.search(Q, k)
+    assert np.array_equal(I, I2) and np.array_equal(D.view(np.uint32), D2.view(np.uint32))
+
+
 @pytest.mark.parametrize("n,d,nq,k", [(60000, 768, 64, 100), (120000, 96, 200, 1000), (50000, 768, 1, 10)])
 def test_search_equals_a_bf16_index_of_the_same_values(R, n, d, nq, k):
     X, Q = gaussian(8, (n, d)), gaussian(9, (nq, d))
