@@ -1366,25 +1366,15 @@ constexpr int MX_MAX_K = IPX_MAX_K;      // deepest list of a search
 constexpr int MX_SLICE = 4096;           // queries per pass of a search (bounds the workspace)
 constexpr int64_t MX_WHOLE = 4096, MX_WHOLE_PAIRS = 1 << 20;      // scan_mx4_path: rows, rows x queries scored without a scan
 
-// How a product runs: 32-query groups per workgroup, splits of the corpus, whether the query block stays in LDS; the
-// groups of a wave tile and the waves of a workgroup.
-#ifndef MXS_RG1
-#define MXS_RG1 2
-#define MXS_W1 16
-#endif
-#ifndef MXS_RG2
-#define MXS_RG2 2
-#define MXS_W2 8
-#endif
-#ifndef MXF_RG1
-#define MXF_RG1 4
-#define MXF_W1 8
-#endif
-#ifndef MXF_RG2
-#define MXF_RG2 4
-#define MXF_W2 8
-#endif
+// How a product runs: 32-query groups per workgroup (cg), splits of the corpus, whether the query block stays in LDS; the
+// row groups of a wave tile and the waves of a workgroup.
 struct MxGeom { int cg, rg, waves, nqb, S, lds; bool resident; int64_t ntiles, rounds; };
+// Tiles. Scores: small ones, whose outputs leave while the other waves multiply (2 groups, 16 waves at 32 queries; 8 at 64;
+// 4 groups, 8 waves: 333 x 50021 x 100 32 instead of 27 us, large ones alike). Search, several query blocks: bound by the matrix
+// cores, 4 groups (1000 queries x 500k x 768: scan 402 us; 2 groups 424, with 6 waves 563). Search, one block: bound by HBM,
+// and what 256 CUs x 8 waves x 16 KB have in flight is the size of the L2s, so that lines are gone before their second half
+// is read; 2 groups and 4 waves at 32 queries (1.8M x 768: 120 us, 6.1 TB/s; 4 groups, 8 waves 129), 6 waves at 64 (151; 8
+// waves 157; 4 groups, 8 waves 168; 4 waves 170).
 MxGeom mx4_geometry(const ipx_index* ix, int64_t nq, int quad_bytes_per_cg, int mode, int64_t groups) {
     MxGeom g;
     const int room = 160 * 1024 - 1024;
@@ -1395,9 +1385,10 @@ MxGeom mx4_geometry(const ipx_index* ix, int64_t nq, int quad_bytes_per_cg, int 
     g.resident = g.cg * whole <= room;
     if (!g.resident) g.cg = nq <= 32 ? 1 : 2;
     g.lds = g.resident ? whole * g.cg : quad_bytes_per_cg * g.cg;
-    g.rg = mode == ipx::MX_SEARCH ? (g.cg == 1 ? MXF_RG1 : MXF_RG2) : (g.cg == 1 ? MXS_RG1 : MXS_RG2);
-    g.waves = mode == ipx::MX_SEARCH ? (g.cg == 1 ? MXF_W1 : MXF_W2) : (g.cg == 1 ? MXS_W1 : MXS_W2);
     g.nqb = (int)((nq + 32 * g.cg - 1) / (32 * g.cg));
+    const bool stream = mode == ipx::MX_SEARCH && g.nqb == 1 && g.resident;
+    g.rg = mode == ipx::MX_SCORES || stream ? 2 : 4;
+    g.waves = mode == ipx::MX_SCORES ? (g.cg == 1 ? 16 : 8) : stream ? (g.cg == 1 ? 4 : 6) : 8;
     g.ntiles = (groups + g.rg - 1) / g.rg;
     // (a short corpus goes to as many CUs as it has tiles: a tile per wave of few workgroups leaves the matrix cores of the
     // other CUs idle — 100k x 768, one query: 19 us on 98 CUs)
@@ -1410,11 +1401,14 @@ template <int PARTS, int FMT, int MODE>
 int launch_mx4_product(const MxGeom& g, ipx::MxParams p, hipStream_t st) {
     p.S = g.S;
     p.ntiles = g.ntiles;
-    constexpr bool SEARCH = MODE == ipx::MX_SEARCH;
-    constexpr int R1 = SEARCH ? MXF_RG1 : MXS_RG1, R2 = SEARCH ? MXF_RG2 : MXS_RG2, W1 = SEARCH ? MXF_W1 : MXS_W1, W2 = SEARCH ? MXF_W2 : MXS_W2;
-    void (*kern)(const ipx::MxParams) =
-        g.resident ? (g.cg == 1 ? ipx::mx4_product_kernel<1, R1, W1, PARTS, FMT, MODE, true> : ipx::mx4_product_kernel<2, R2, W2, PARTS, FMT, MODE, true>)
-                   : (g.cg == 1 ? ipx::mx4_product_kernel<1, R1, W1, PARTS, FMT, MODE, false> : ipx::mx4_product_kernel<2, R2, W2, PARTS, FMT, MODE, false>);
+    void (*kern)(const ipx::MxParams) = nullptr;
+    if constexpr (MODE == ipx::MX_SCORES)
+        kern = g.resident ? (g.cg == 1 ? ipx::mx4_product_kernel<1, 2, 16, PARTS, FMT, MODE, true> : ipx::mx4_product_kernel<2, 2, 8, PARTS, FMT, MODE, true>)
+                          : (g.cg == 1 ? ipx::mx4_product_kernel<1, 2, 16, PARTS, FMT, MODE, false> : ipx::mx4_product_kernel<2, 2, 8, PARTS, FMT, MODE, false>);
+    else
+        kern = g.rg == 2    ? (g.cg == 1 ? ipx::mx4_product_kernel<1, 2, 4, PARTS, FMT, MODE, true> : ipx::mx4_product_kernel<2, 2, 6, PARTS, FMT, MODE, true>)
+               : g.resident ? (g.cg == 1 ? ipx::mx4_product_kernel<1, 4, 8, PARTS, FMT, MODE, true> : ipx::mx4_product_kernel<2, 4, 8, PARTS, FMT, MODE, true>)
+                            : (g.cg == 1 ? ipx::mx4_product_kernel<1, 4, 8, PARTS, FMT, MODE, false> : ipx::mx4_product_kernel<2, 4, 8, PARTS, FMT, MODE, false>);
     if (int rc = ensure_dynamic_lds((const void*)kern, std::max(g.lds, 64 * 1024 + 1))) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)(g.nqb * g.S)), dim3(g.waves * 64), g.lds, st, p);
     IPX_HIP(hipGetLastError());
@@ -1604,7 +1598,17 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
         rp.k = k;
         rp.kc = 0;
         rp.P = next_pow2((int)ix->ntotal);
-        return launch_rescore(rp, nq, st);
+        if (ix->timing) {                     // (one kernel: its time counts as the scan's)
+            IPX_HIP(hipEventRecord(ix->ev[0], st));
+            IPX_HIP(hipEventRecord(ix->ev[1], st));
+        }
+        if (int rc = launch_rescore(rp, nq, st)) return rc;
+        if (ix->timing) IPX_HIP(hipEventRecord(ix->ev[2], st));
+        ix->ev_valid = ix->timing;
+        ix->last_wgs = (int)nq;
+        ix->last_S = 1;
+        ix->last_cap = 0;
+        return 0;
     }
     const int kc0 = ix->force_kc > 0 ? ix->force_kc : (int)((int64_t)std::max(128, k + k / 4) * ix->kc_boost / 8);
     const int kc = std::min(std::max(kc0, k), MAX_KC);

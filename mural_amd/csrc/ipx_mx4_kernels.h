@@ -471,8 +471,8 @@ __device__ __forceinline__ void static_for(F&& f) {
 // One wave: 32 RG rows x BQ = 32 CG queries; WAVES waves a workgroup, which share the query block in LDS and
 // nothing else: while the whole block fits (RESIDENT) the main loop has no barrier. The loop steps through quads of K-sets
 // (256 elements), the quads of a tile and on to the next tile. A K-set's row operands wait in registers: the slot of a
-// K-set is loaded again, for the next quad, as soon as its last MFMA is issued, so four K-sets are in flight (RG = 4: 16 KiB
-// a wave). The query operands of the next part are read from LDS while the current part is multiplied: RG x CG MFMAs
+// K-set is loaded again, for the next quad, as soon as its last MFMA (and its neighbour's) is issued, so three to four K-sets
+// are in flight (RG = 4: 16 KiB a wave). The query operands of the next part are read from LDS while the current part is multiplied: RG x CG MFMAs
 // per CG reads of 24 bytes a lane.
 // Tiles are dealt round-robin over a query block's S workgroups, then over their waves. When the query block does not fit (long
 // vectors), its quads go through LDS one at a time, all waves in step.
