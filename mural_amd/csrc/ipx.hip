@@ -1362,6 +1362,10 @@ int scan_bf16_path(ipx_index* ix, const float* dq, const float* dw, int A, int l
 // ---- mx4 rows (storage 3) -------------------------------------------------------------------------------------
 constexpr int MX_PARTS_SEARCH = 2;       // E2M3 parts per query in the scan: what they leave out enters the margin rule
 constexpr int MX_PARTS_SCORES = 5;       // ... in ipx_scores: as exact as fp32
+// ipx_scores: up to this many queries are packed by the product kernel itself, in every workgroup, not by a kernel before it
+// (with it -> without, us; 1 query: 1000 x 768 rows 13.9 -> 9.4, 100k 17.3 -> 15.0, 1M 90 -> 91; 4 queries: 13.8 -> 10.9,
+// 17.3 -> 16.1, 97 -> 96.5; 8 queries: 13.9 -> 12.9, 17.9 -> 18.3, 103 -> 108)
+constexpr int MX_PACK_HERE = 4;
 constexpr int MX_MAX_K = IPX_MAX_K;      // deepest list of a search
 constexpr int MX_SLICE = 4096;           // queries per pass of a search (bounds the workspace)
 constexpr int64_t MX_WHOLE = 4096, MX_WHOLE_PAIRS = 1 << 20;      // scan_mx4_path: rows, rows x queries scored without a scan
@@ -1674,16 +1678,19 @@ int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sca
     const int quad1 = MX_PARTS_SCORES * ipx::mx_part_bytes<ipx::MX_E2M3>(32);
     const MxGeom g = mx4_geometry(ix, nq, quad1, ipx::MX_SCORES, groups);
     p.gstep = g.rg;
-    if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
-    if (int rc = ix->mxq.ensure((size_t)nq * sizeof(ipx::MxQueryInfo))) return rc;
-    hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)nq), dim3(256), 0, st, dq, q_dtype, ix->d, MX_PARTS_SCORES,
-                       32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr, (float*)nullptr,
-                       (uint32_t*)nullptr);
-    IPX_HIP(hipGetLastError());
-    p.Q = (const uint8_t*)ix->Qp.p;
     p.q = dq;
     p.q_dtype = q_dtype;
-    p.info = (const ipx::MxQueryInfo*)ix->mxq.p;
+    p.pack_here = g.resident && nq <= MX_PACK_HERE;
+    if (!p.pack_here) {
+        if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
+        if (int rc = ix->mxq.ensure((size_t)nq * sizeof(ipx::MxQueryInfo))) return rc;
+        hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)nq), dim3(256), 0, st, dq, q_dtype, ix->d, MX_PARTS_SCORES,
+                           32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr, (float*)nullptr,
+                           (uint32_t*)nullptr);
+        IPX_HIP(hipGetLastError());
+        p.Q = (const uint8_t*)ix->Qp.p;
+        p.info = (const ipx::MxQueryInfo*)ix->mxq.p;
+    }
     return launch_mx4_product<MX_PARTS_SCORES, ipx::MX_E2M3, ipx::MX_SCORES>(g, p, st);
 }
 

@@ -319,6 +319,46 @@ struct MxQueryInfo {      // of one query
     float restsq;         // |q - sum of its parts|^2        very small elements vanish, the bounds they stand for must not)
 };
 
+// One lane's four elements of block b (K-set b >> 1, half b & 1) of query ql into its block; the eight lanes of a block are
+// neighbours, `sub` is the lane's number among them. x: the elements, then what the parts leave (0 in a block
+// with a NaN or an infinity, whose scales are NaN).
+__device__ __forceinline__ void mx_pack_lane(float (&x)[4], int b, int sub, int parts, int bq, int ql, uint8_t* block) {
+    const int part_bytes = bq * 200, quad = b >> 3, j = (b >> 1) & 3, h = b & 1;
+    bool bad = false;
+    for (int p = 0; p < parts; ++p) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));       // quad_perm [1,0,3,2]
+        top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));       // quad_perm [2,3,0,1]
+        top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xF, 0xF, true));      // row_half_mirror
+        bad |= top >= 0x7f800000u;                                  // NaN / inf: the block's scales are NaN
+        // smallest s in [-127, 125] with the largest magnitude <= 7.5 x 2^s
+        const int s = max((int)(top >> 23) - 129 + ((top & 0x7fffffu) > 0x700000u ? 1 : 0), -127);
+        const float inv = __uint_as_float((uint32_t)(127 - s) << 23), scale = mx_scale_f32((uint32_t)(s + 127));
+        uint32_t bits = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (bad) { x[e] = 0.f; continue; }
+            const float a = fabsf(x[e]) * inv;
+            // codes count steps of 1/8 below 2, 1/4 below 4, 1/2 up to 7.5
+            const float per = a < 2.f ? 8.f : a < 4.f ? 4.f : 2.f, step = a < 2.f ? 0.125f : a < 4.f ? 0.25f : 0.5f;
+            const float c = rintf(a * per), v = c * step;
+            const uint32_t neg = __float_as_uint(x[e]) >> 31, code = (uint32_t)((int)c + (a < 2.f ? 0 : a < 4.f ? 8 : 16));
+            bits |= (code | neg << 5) << (6 * e);
+            x[e] -= (neg ? -v : v) * scale;                         // exact: both are multiples of x's last place
+        }
+        uint8_t* part = block + ((size_t)quad * parts + p) * part_bytes;
+        // the lane's 24 bits are bytes 3 sub .. 3 sub + 2 of the block's 24
+#pragma unroll
+        for (int y = 0; y < 3; ++y) {
+            const int at = sub * 3 + y;
+            part[at < 16 ? ((j * 2 + h) * bq + ql) * 16 + at : bq * 128 + ((j * 2 + h) * bq + ql) * 8 + (at - 16)] = (uint8_t)(bits >> (8 * y));
+        }
+        if (sub == 0) part[bq * 192 + (h * bq + ql) * 4 + j] = bad ? 255 : (uint8_t)(s + 127);
+    }
+}
+
 // One workgroup per query. Eight lanes per block, four elements each. With `tau`, the
 // state of a search without a floor is written too: every row that scores a number is a hit.
 __global__ void __launch_bounds__(256)
@@ -328,11 +368,10 @@ mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int d, int part
     const int tid = threadIdx.x, lane = tid & 63;
     bool nonzero = false;
     const int64_t q = blockIdx.x;
-    const int part_bytes = bq * 200;
-    uint8_t* block = dst + (size_t)(q / bq) * nkq * parts * part_bytes;
+    uint8_t* block = dst + (size_t)(q / bq) * nkq * parts * bq * 200;
     const int ql = (int)(q % bq), sub = tid & 7;
     float ss = 0.f, rr = 0.f;
-    for (int b = tid >> 3; b < nkq * 8; b += 32) {                      // block b: K-set b >> 1, half b & 1
+    for (int b = tid >> 3; b < nkq * 8; b += 32) {
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -341,41 +380,7 @@ mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int d, int part
             ss = fmaf(x[e], x[e], ss);
             nonzero |= x[e] != 0.f;
         }
-        const int quad = b >> 3, j = (b >> 1) & 3, h = b & 1;
-        for (int p = 0; p < parts; ++p) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));       // quad_perm [1,0,3,2]
-            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));       // quad_perm [2,3,0,1]
-            top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xF, 0xF, true));      // row_half_mirror
-            const bool bad = top >= 0x7f800000u;                        // NaN / inf: the block's scale is NaN
-            // smallest s in [-127, 125] with the largest magnitude <= 7.5 x 2^s
-            const int s = max((int)(top >> 23) - 129 + ((top & 0x7fffffu) > 0x700000u ? 1 : 0), -127);
-            const float inv = __uint_as_float((uint32_t)(127 - s) << 23), scale = mx_scale_f32((uint32_t)(s + 127));
-            uint32_t bits = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (bad) { x[e] = 0.f; continue; }
-                const float a = fabsf(x[e]) * inv;
-                // codes count steps of 1/8 below 2, 1/4 below 4, 1/2 up to 7.5
-                const float per = a < 2.f ? 8.f : a < 4.f ? 4.f : 2.f, step = a < 2.f ? 0.125f : a < 4.f ? 0.25f : 0.5f;
-                const float c = rintf(a * per), v = c * step;
-                const uint32_t neg = __float_as_uint(x[e]) >> 31, code = (uint32_t)((int)c + (a < 2.f ? 0 : a < 4.f ? 8 : 16));
-                bits |= (code | neg << 5) << (6 * e);
-                x[e] -= (neg ? -v : v) * scale;                         // exact: both are multiples of x's last place
-            }
-            uint8_t* part = block + ((size_t)quad * parts + p) * part_bytes;
-            // the lane's 24 bits are bytes 3 sub .. 3 sub + 2 of the block's 24
-#pragma unroll
-            for (int y = 0; y < 3; ++y) {
-                const int at = sub * 3 + y;
-                uint8_t* o = at < 16 ? part + ((j * 2 + h) * bq + ql) * 16 + at
-                                     : part + bq * 128 + ((j * 2 + h) * bq + ql) * 8 + (at - 16);
-                *o = (uint8_t)(bits >> (8 * y));
-            }
-            if (sub == 0) part[bq * 192 + (h * bq + ql) * 4 + j] = bad ? 255 : (uint8_t)(s + 127);
-        }
+        mx_pack_lane(x, b, sub, parts, bq, ql, block);
 #pragma unroll
         for (int e = 0; e < 4; ++e) rr = fmaf(x[e], x[e], rr);
     }
@@ -434,6 +439,7 @@ struct MxParams {
     int64_t ld, row0, n;         // columns 0 .. n - 1 are rows row0 ..; row0 < 0: column = 32 RG t + row of the tile
     const void* q;               // the caller's queries (recomputation of those with NaN / inf elements), or null
     int q_dtype;
+    int pack_here;               // the queries (one block) are not packed yet: every workgroup does it
     const MxQueryInfo* info;
     // search
     const float* tau;            // [nq] floor: a hit scores above it, or equals it with row < row_below
@@ -510,7 +516,7 @@ mx4_product_kernel(const MxParams p) {
             below[c] = q < p.nq ? p.row_below[q] : 0;
             at[c] = list_start(c);
         }
-    } else if (p.q) {
+    } else if (p.q && !p.pack_here) {
 #pragma unroll
         for (int c = 0; c < CG; ++c) {
             const int q = qb * BQ + c * 32 + l31;
@@ -524,8 +530,30 @@ mx4_product_kernel(const MxParams p) {
 #pragma unroll 4
         for (int i = tid; i < quads * (QUAD / 16); i += THREADS) ((uint4*)smem)[i] = s[i];
     };
-    if constexpr (RESIDENT) stage(0, p.nkq);
+    __shared__ int s_bad;               // a bit per query to be scored in fp32 (packed here)
+    if (MODE == MX_SCORES && FMT == MX_E2M3 && RESIDENT && p.pack_here) {
+        // very few queries: packing them in every workgroup is shorter than a launch before this one (times below MX_PACK_HERE)
+        if (tid == 0) s_bad = 0;
+        __syncthreads();
+        const int sub = tid & 7;
+        for (int i = tid >> 3; i < p.nq * p.nkq * 8; i += THREADS / 8) {
+            const int ql = i / (p.nkq * 8), b = i - ql * (p.nkq * 8);
+            bool exact = false;
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int at = b * 32 + sub * 4 + e;
+                x[e] = at < p.d ? load_as_f32(p.q, p.q_dtype, (int64_t)ql * p.d + at) : 0.f;
+                exact |= !(fabsf(x[e]) < 0x1p63f);              // not finite, or its square may not be
+            }
+            mx_pack_lane(x, b, sub, PARTS, BQ, ql, (uint8_t*)smem);
+            if (exact) atomicOr(&s_bad, 1 << ql);
+        }
+    } else if constexpr (RESIDENT) {
+        stage(0, p.nkq);
+    }
     __syncthreads();
+    if (MODE == MX_SCORES && FMT == MX_E2M3 && RESIDENT && p.pack_here) redo = s_bad;
 
     const int64_t per_round = (int64_t)p.S * WAVES;
     const int64_t rounds = (p.ntiles + per_round - 1) / per_round;
@@ -602,7 +630,7 @@ mx4_product_kernel(const MxParams p) {
 #pragma unroll 1
                     for (int i = 0; i < BQ; ++i) {
                         const int q = qb * BQ + i;
-                        if (((i >> 2) & 1) == h && q < p.nq && !(p.info[q].sumsq <= FLT_MAX))
+                        if (((i >> 2) & 1) == h && q < p.nq && (p.pack_here ? s_bad >> i & 1 : !(p.info[q].sumsq <= FLT_MAX)))
                             p.out[(size_t)q * p.ld + col] = mx4_plain_dot(p, q, (g + r) * 32 + l31);
                     }
             }
