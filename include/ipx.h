@@ -18,7 +18,8 @@
  *     without synchronising. With a bf16 copy or 4-bit rows (storage 1, 2, 3) ipx_search /
  *     ipx_search_aspect / ipx_search_pooled read back one flag word per query
  *     after the rescoring pass (which queries the margin rule sends to a repeat
- *     pass) and so synchronise the stream once per pass before they return;
+ *     pass) and so synchronise the stream once per pass before they return (storage 3: not on an index of up to 4096
+ *     rows with nq * rows <= 2^20, which takes one launch);
  *     ipx_merge_topk synchronises when a list exceeds IPX_MAX_K entries.
  *   - an index serves one call at a time: its scratch buffers, timing events
  *     and last-search statistics are per index, not per call. Concurrent
@@ -179,7 +180,11 @@ int ipx_add_mx4(ipx_index* idx, const uint8_t* codes, const uint8_t* scales, int
 /* out[i][j] = <q_i, row row0 + j of the index>, fp32 [nq, n], storage 3 only. q: [nq, d] of q_dtype, taken to within 2^-20
  * of the largest magnitude of each block of 32 elements (in practice 2^-24), products and sums in fp32; a query with a
  * NaN or an infinity is multiplied element by element. ipx_scores_mx4: queries in mx4, products exact.
- * With on_device != 0 stream-ordered; the first call of a size allocates the index's query buffers. */
+ * n < 2^27. With on_device != 0 stream-ordered: never synchronises, and allocates only where more than 4 queries are the
+ * most so far (the index's query buffers).
+ * HIP graphs: run a call of the size once, then capture it (on_device != 0; ipx_lookup likewise). A replay counts as a call
+ * on the index (one at a time) and reads the rows as the index held them when it was captured; adding rows, or larger
+ * calls, later does not disturb it. */
 int ipx_scores(ipx_index* idx, const void* q, int q_dtype, int64_t nq, int64_t row0, int64_t n, float* out,
                int on_device, void* stream);
 int ipx_scores_mx4(ipx_index* idx, const uint8_t* q_codes, const uint8_t* q_scales, int64_t nq, int64_t row0, int64_t n,

@@ -61,9 +61,15 @@ int fail(int code, const std::string& msg) {
 struct DevBuf {
     void* p = nullptr;
     size_t bytes = 0;
+    bool captured = false;          // a graph's kernels use p: a larger buffer replaces it, but it lives on
+    std::vector<void*> old;
     int ensure(size_t need) {
         if (need <= bytes) return 0;
-        if (p) { (void)hipFree(p); p = nullptr; bytes = 0; }
+        if (p) {
+            if (captured) old.push_back(p);
+            else (void)hipFree(p);
+            p = nullptr; bytes = 0; captured = false;
+        }
         hipError_t e = hipMalloc(&p, need);
         if (e != hipSuccess) {
             p = nullptr;
@@ -74,10 +80,19 @@ struct DevBuf {
     }
     void release() {
         if (p) (void)hipFree(p);
+        for (void* o : old) (void)hipFree(o);
+        old.clear();
         p = nullptr;
         bytes = 0;
     }
 };
+
+int is_capturing(hipStream_t st, bool* yes) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    IPX_HIP(hipStreamIsCapturing(st, &status));
+    *yes = status == hipStreamCaptureStatusActive;
+    return 0;
+}
 
 // Makes `device` current for the duration of a call and restores the caller's device afterwards.
 struct DeviceGuard {
@@ -160,6 +175,12 @@ struct ipx_index {
     //          3 = mx4 rows only (ipx_mx4_kernels.h): scaled-MFMA scan, exact rescoring of the 4-bit values
     int storage = 0;
     bool lookups = false;    // ipx_lookup has run on device ids: ipx_check reads its error word too
+    bool rows_captured = false;      // a graph's kernels (ipx_scores, ipx_lookup) read the rows where they lie:
+    std::vector<void*> old_rows;     // ... when the rows move, what they leave lives on
+    void free_rows(void* p) {
+        if (rows_captured) old_rows.push_back(p);
+        else (void)hipFree(p);
+    }
     int nks_h = 0;           // K-stages of 32 bf16
     int64_t cap_tiles_h = 0; // tiles of 256 rows the bf16 buffer holds
     uint16_t* Xh = nullptr;  // packed bf16 corpus (storage 1, 2)
@@ -245,7 +266,7 @@ int grow_corpus(ipx_index* ix, int64_t need_tiles, hipStream_t st) {
         (void)hipFree(nb);
         return fail(IPX_ERR_HIP, std::string("grow corpus: ") + hipGetErrorString(ce));
     }
-    if (ix->Xp) (void)hipFree(ix->Xp);
+    if (ix->Xp) ix->free_rows(ix->Xp);
     ix->Xp = nb;
     ix->cap_tiles = new_tiles;
     return 0;
@@ -272,7 +293,7 @@ int grow_corpus_h(ipx_index* ix, int64_t need_tiles, hipStream_t st) {
         (void)hipFree(nb);
         return fail(IPX_ERR_HIP, std::string("grow bf16 corpus: ") + hipGetErrorString(ce));
     }
-    if (ix->Xh) (void)hipFree(ix->Xh);
+    if (ix->Xh) ix->free_rows(ix->Xh);
     ix->Xh = nb;
     ix->cap_tiles_h = new_tiles;
     return 0;
@@ -306,8 +327,8 @@ int grow_corpus_x(ipx_index* ix, int64_t need_groups, hipStream_t st) {
         (void)hipFree(ns);
         return fail(IPX_ERR_HIP, std::string("grow mx4 corpus: ") + hipGetErrorString(e));
     }
-    if (ix->Xx) (void)hipFree(ix->Xx);
-    if (ix->Xxs) (void)hipFree(ix->Xxs);
+    if (ix->Xx) ix->free_rows(ix->Xx);
+    if (ix->Xxs) ix->free_rows(ix->Xxs);
     ix->Xx = nb;
     ix->Xxs = ns;
     ix->cap_groups_x = want;
@@ -1366,6 +1387,7 @@ constexpr int MX_PARTS_SCORES = 5;       // ... in ipx_scores: as exact as fp32
 // (with it -> without, us; 1 query: 1000 x 768 rows 13.9 -> 9.4, 100k 17.3 -> 15.0, 1M 90 -> 91; 4 queries: 13.8 -> 10.9,
 // 17.3 -> 16.1, 97 -> 96.5; 8 queries: 13.9 -> 12.9, 17.9 -> 18.3, 103 -> 108)
 constexpr int MX_PACK_HERE = 4;
+constexpr int64_t MX_SCORES_SLICE = 1 << 18;      // queries per pass of ipx_scores: bounds the workspace (4 KB a query of 768) and a launch's threads
 constexpr int MX_MAX_K = IPX_MAX_K;      // deepest list of a search
 constexpr int MX_SLICE = 4096;           // queries per pass of a search (bounds the workspace)
 constexpr int64_t MX_WHOLE = 4096, MX_WHOLE_PAIRS = 1 << 20;      // scan_mx4_path: rows, rows x queries scored without a scan
@@ -1576,8 +1598,6 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
     // synchronisation). 3 queries, 999 rows of 100: 43 us for the passes below. The limit: 16 chains of 64 rows keep a CU busy for about
     // as long as the passes take.
     if (ix->ntotal <= MX_WHOLE && nq * ix->ntotal <= MX_WHOLE_PAIRS && ix->force_kc == 0) {
-        if (int rc = ix->mxq.ensure((size_t)nq * sizeof(ipx::MxQueryInfo))) return rc;
-        if (int rc = ix->flags.ensure((size_t)nq * sizeof(int))) return rc;
         ipx::RescoreParams rp;
         rp.candD = nullptr;
         rp.candI = nullptr;
@@ -1589,7 +1609,7 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
         rp.maxsq = (const uint32_t*)ix->maxsq.p;
         rp.outD = dD;
         rp.outI = dI;
-        rp.flags = (int*)ix->flags.p;
+        rp.flags = nullptr;
         rp.err = nullptr;
         rp.outl_count = nullptr;
         rp.shared_list = 0;
@@ -1650,9 +1670,9 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
     return 0;
 }
 
-// S = Q X^T over rows [row0, row0 + n) of an mx4 index; out: device, [nq][n].
-int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_scales, int64_t nq, int64_t row0, int64_t n, float* out,
-                hipStream_t st) {
+// S = Q X^T over rows [row0, row0 + n) of an mx4 index; out: device, [nq][n]. nq <= MX_SCORES_SLICE.
+int scores_slice(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_scales, int64_t nq, int64_t row0, int64_t n, float* out,
+                 bool captured, hipStream_t st) {
     ipx::MxParams p = {};
     mx4_rows(ix, p);
     // (a tile is a power of two of groups and the buffers end behind eight: groups up to a tile's end exist)
@@ -1672,6 +1692,7 @@ int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sca
         hipLaunchKernelGGL(ipx::mx4_pack_codes_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, (const uint8_t*)dq,
                            q_scales, ix->d, 32 * g.cg, ix->nkq_x, total, (uint8_t*)ix->Qp.p);
         IPX_HIP(hipGetLastError());
+        ix->Qp.captured |= captured;
         p.Q = (const uint8_t*)ix->Qp.p;
         return launch_mx4_product<1, ipx::MX_E2M1, ipx::MX_SCORES>(g, p, st);
     }
@@ -1688,10 +1709,25 @@ int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sca
                            32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr, (float*)nullptr,
                            (uint32_t*)nullptr);
         IPX_HIP(hipGetLastError());
+        ix->Qp.captured |= captured;
+        ix->mxq.captured |= captured;
         p.Q = (const uint8_t*)ix->Qp.p;
         p.info = (const ipx::MxQueryInfo*)ix->mxq.p;
     }
     return launch_mx4_product<MX_PARTS_SCORES, ipx::MX_E2M3, ipx::MX_SCORES>(g, p, st);
+}
+
+int scores_path(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_scales, int64_t nq, int64_t row0, int64_t n, float* out,
+                hipStream_t st) {
+    bool captured = false;
+    if (int rc = is_capturing(st, &captured)) return rc;
+    ix->rows_captured |= captured;
+    const size_t nb = (size_t)(ix->d + 31) / 32, qbytes = q_scales ? nb * 16 : ix->d * dtype_size(q_dtype);
+    for (int64_t q0 = 0; q0 < nq; q0 += MX_SCORES_SLICE)
+        if (int rc = scores_slice(ix, (const char*)dq + (size_t)q0 * qbytes, q_dtype, q_scales ? q_scales + (size_t)q0 * nb : nullptr,
+                                  std::min(MX_SCORES_SLICE, nq - q0), row0, n, out + (size_t)q0 * n, captured, st))
+            return rc;
+    return 0;
 }
 
 // Shared body of ipx_search / ipx_search_aspect. q_src is [nq, d] (A == 0) or [nq, A, d].
@@ -1926,6 +1962,7 @@ int ipx_destroy(ipx_index* ix) {
     if (ix->Xh) (void)hipFree(ix->Xh);
     if (ix->Xx) (void)hipFree(ix->Xx);
     if (ix->Xxs) (void)hipFree(ix->Xxs);
+    for (void* p : ix->old_rows) (void)hipFree(p);
     for (DevBuf* b : {&ix->Qp, &ix->cand, &ix->partD, &ix->partI, &ix->err, &ix->stageIn, &ix->stageQ, &ix->stageW,
                       &ix->outD, &ix->outI, &ix->trace, &ix->pub, &ix->maxsq, &ix->outl, &ix->olist, &ix->sideD, &ix->sideI, &ix->qfused, &ix->candD, &ix->candI, &ix->deepD, &ix->deepI, &ix->ceilD, &ix->ceilI, &ix->deepK, &ix->deepN,
                       &ix->flags, &ix->sel, &ix->qsel, &ix->selD, &ix->selI, &ix->poolH, &ix->poolW, &ix->poolQ, &ix->mxq, &ix->mxs})
@@ -2129,6 +2166,9 @@ int ipx_lookup(ipx_index* ix, const int64_t* ids, int64_t n, const float* scale,
         ds = scale ? (const float*)((char*)ix->stageQ.p + ib) : nullptr;
         dout = (char*)ix->outD.p;
     } else {
+        bool captured = false;
+        if (int rc = is_capturing(st, &captured)) return rc;
+        ix->rows_captured |= captured;
         ix->lookups = true;
     }
     const int xfmt = ix->storage == 3 ? 2 : ix->storage == 2 ? 1 : 0;
@@ -2603,9 +2643,10 @@ int ipx_check(ipx_index* ix, void* stream) {
     }
     if (ix->lookups) {
         int bad = 0;
-        IPX_HIP(hipMemcpy(&bad, (int*)ix->err.p + LOOKUP_ERR, sizeof(int), hipMemcpyDeviceToHost));
+        IPX_HIP(hipMemcpyAsync(&bad, (int*)ix->err.p + LOOKUP_ERR, sizeof(int), hipMemcpyDeviceToHost, st));
+        IPX_HIP(hipStreamSynchronize(st));
         if (bad) {
-            (void)hipMemset((int*)ix->err.p + LOOKUP_ERR, 0, sizeof(int));
+            (void)hipMemsetAsync((int*)ix->err.p + LOOKUP_ERR, 0, sizeof(int), st);
             return fail(IPX_ERR_ARG, "lookup: an id was neither -1 nor a row of the index (its row was filled with zeros)");
         }
     }

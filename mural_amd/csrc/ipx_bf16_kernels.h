@@ -902,7 +902,7 @@ struct RescoreParams {
     const uint32_t* maxsq;   // float bits of max_x |x|^2 and max_x |x - bf16(x)|^2
     float* outD;             // [nq][k]
     int64_t* outI;           // [nq][k]
-    int* flags;              // [nq] (+ 1 when err is given)
+    int* flags;              // [nq] (+ 1 when err is given); not written with all_rows
     const int* err;          // optional: the scan's error word, copied to flags[nq] so that one readback brings both
     const int* outl_count;   // optional (with err): the index's outlier-row count, copied to flags[nq + 1]
     const int* todo = nullptr;   // optional [nq]: 1 = merge_pool_kernel left this query without a list (pool overflow)
@@ -1111,7 +1111,7 @@ rescore_kernel(const RescoreParams p) {
         }
         s_m = m;
         s_post = post;
-        p.flags[qi] = flag;
+        if (!whole) p.flags[qi] = flag;
         if (p.err && qi == 0) {                            // the scans are done: same stream
             p.flags[p.nq] = *p.err;
             p.flags[p.nq + 1] = p.outl_count ? *p.outl_count : 0;

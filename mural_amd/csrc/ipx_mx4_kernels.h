@@ -5,7 +5,7 @@
 // (sign, two exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6) of element / 2^s, rounded to nearest, ties to
 // the even code, magnitudes beyond 6 to 6. A block with a NaN or an infinity has the scale byte 255 and stands for NaNs.
 // A value code x 2^s has two significant bits and an exponent in fp32's (and bf16's) range: it is exact in both.
-// 17 bytes per 32 elements: 408 bytes for 768 of them, where fp32 takes 3072 and bf16 1536.
+// 17 bytes per 32 elements: 408 bytes for 768 of them, 0.13 of fp32.
 //
 // External form: codes [n][nb][16] bytes (element 2i of a block in the low nibble of byte i), scales [n][nb] bytes,
 // nb = ceil(d / 32). Codes behind element d are 0.

@@ -415,6 +415,65 @@ def test_on_another_stream_and_in_a_graph(R, mx4, torch):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("storage", ["mx4", "bf16", "f32"])
+def test_a_graph_outlives_larger_calls_and_added_rows(R, mx4, torch, storage):
+    """Buffers that a captured call uses are replaced, not freed, when a later call needs larger ones."""
+    X = torch.from_numpy(gaussian(101, (1500, 96))).cuda()
+    ix = R.FlatIPIndex(96, storage=storage)
+    ix.add(X)
+    q = torch.from_numpy(gaussian(102, (9, 96))).cuda()
+    codes, scales = mx4.quantize(q)
+    ids = torch.arange(1499, -1, -3, device="cuda")
+
+    def work():
+        if storage != "mx4":
+            return (ix.lookup(ids),)
+        return ix.scores(q, 0, 1500), ix.scores(q[:2], 0, 1500), ix.scores_mx4(codes, scales, 0, 1500), ix.lookup(ids)
+
+    first = work()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for grow in range(3):
+        for o in out:
+            o.fill_(-7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, first))
+        ix.add(torch.from_numpy(gaussian(103 + grow, (3000 << grow, 96))).cuda())
+        if storage == "mx4":
+            ix.scores(torch.from_numpy(gaussian(104, (2000, 96))).cuda())
+        assert all(torch.equal(a, b) for a, b in zip(work(), first))
+
+
+def test_scores_of_a_query_do_not_depend_on_the_others(R, torch):
+    """Up to four queries are packed by the product kernel, more by a kernel before it: the same bits."""
+    X, q = gaussian(105, (700, 300)), gaussian(106, (40, 300))
+    q[1, 7], q[2, 299], q[3] = np.inf, np.nan, q[3] * np.float32(2.0 ** 100)
+    ix = index(R, X)
+    tq = torch.from_numpy(q).cuda()
+    full = ix.scores(tq).cpu().numpy()
+    for n in (1, 2, 3, 4, 5, 33):
+        for lo in (0, 1, 7):
+            assert np.array_equal(ix.scores(tq[lo:lo + n]).cpu().numpy(), full[lo:lo + n], equal_nan=True)
+
+
+def test_scores_of_very_many_queries(R, mx4, torch):
+    """More queries than one pass takes."""
+    n = (1 << 18) + 70
+    X = gaussian(107, (21, 40))
+    ix = index(R, X)
+    q = gaussian(108, (n, 40))
+    tq = torch.from_numpy(q).cuda()
+    Xr = M.dequantize(*M.quantize(X), 40)
+    S = ix.scores(tq).cpu().numpy()
+    assert (np.abs(S - q.astype(np.float64) @ Xr.astype(np.float64).T) <= score_bound(q, Xr)).all()
+    codes, scales = mx4.quantize(tq)
+    S = ix.scores_mx4(codes, scales, 1, 20)
+    for lo in (0, (1 << 18) - 40, n - 70):
+        assert torch.equal(S[lo:lo + 70], ix.scores_mx4(codes[lo:lo + 70], scales[lo:lo + 70], 1, 20))
+
+
 def test_storage_rules(R, mx4):
     from mural_amd import _lib
     ix = R.FlatIPIndex(64, storage="mx4")
