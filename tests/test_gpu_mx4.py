@@ -474,6 +474,30 @@ def test_scores_of_very_many_queries(R, mx4, torch):
         assert torch.equal(S[lo:lo + 70], ix.scores_mx4(codes[lo:lo + 70], scales[lo:lo + 70], 1, 20))
 
 
+def test_offsets_beyond_32_bits(R, mx4, torch):
+    """An index of 4.6 GB and a score matrix of 5 GB: the last rows are found where they are."""
+    d, n, step = 2048, 4300000, 430000
+    g = torch.Generator(device="cuda").manual_seed(5)
+    ix = R.FlatIPIndex(d, storage="mx4")
+    for lo in range(0, n, step):
+        x = torch.randn((step, d), generator=g, device="cuda", dtype=torch.float16)
+        ix.add(x)
+    tail = x[-300:].float()                        # rows n - 300 ..
+    want = mx4.dequantize(*mx4.quantize(tail), d)
+    ids = torch.arange(n - 300, n, device="cuda")
+    assert torch.equal(ix.lookup(ids), want)
+    D, I = ix.search(tail, 3)
+    assert torch.equal(I[:, 0], ids)
+    S = ix.scores(tail)
+    Q, X = tail.cpu().numpy(), want.cpu().numpy()
+    bound = score_bound(Q, X)
+    ref = Q.astype(np.float64) @ X.astype(np.float64).T
+    assert (np.abs(S[:, n - 300:].cpu().numpy() - ref) <= bound).all()
+    assert torch.equal(S[:, n - 300:], ix.scores(tail, n - 300))
+    assert torch.equal(S[:, 77:99], ix.scores(tail, 77, 22))
+    assert (np.abs(D[:, 0].cpu().numpy() - np.diag(ref)) <= np.diag(bound)).all()
+
+
 def test_storage_rules(R, mx4):
     from mural_amd import _lib
     ix = R.FlatIPIndex(64, storage="mx4")
