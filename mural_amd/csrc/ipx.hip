@@ -1670,6 +1670,12 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
     return 0;
 }
 
+// Scores beyond the size of the last cache (256 MB), in whole lines, are stored past the caches: what would be kept of them is gone
+// before anybody reads it, and the lines they drive out are the rows. Kept -> past, us: mx4 queries, 8192 x 32768 332 -> 242,
+// 1000 x 100k (400 MB) 144 -> 93, fp32 queries 245 -> 217; 1000 x 32768 (131 MB) 33 -> 38, with a reduction behind it 58 -> 69.
+// Parts of lines cost more that way (333 x 50021: kept 28, past 42).
+constexpr size_t MX_KEPT_BYTES = (size_t)256 << 20;
+
 // S = Q X^T over rows [row0, row0 + n) of an mx4 index; out: device, [nq][n]. nq <= MX_SCORES_SLICE.
 int scores_slice(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_scales, int64_t nq, int64_t row0, int64_t n, float* out,
                  bool captured, hipStream_t st) {
@@ -1683,6 +1689,7 @@ int scores_slice(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sc
     p.ld = n;
     p.row0 = row0;
     p.n = n;
+    p.past = (size_t)nq * n * 4 >= MX_KEPT_BYTES && n % 32 == 0 && row0 % 32 == 0 && ((uintptr_t)out & 127) == 0;
     if (q_scales) {
         const int quad1 = ipx::mx_part_bytes<ipx::MX_E2M1>(32);
         const MxGeom g = mx4_geometry(ix, nq, quad1, ipx::MX_SCORES, groups);

@@ -437,6 +437,7 @@ struct MxParams {
     // scores
     float* out;                  // [nq][ld]
     int64_t ld, row0, n;         // columns 0 .. n - 1 are rows row0 ..; row0 < 0: column = 32 RG t + row of the tile
+    int past;                    // the output passes the caches by; its tiles' columns are whole lines
     const void* q;               // the caller's queries (recomputation of those with NaN / inf elements), or null
     int q_dtype;
     int pack_here;               // the queries (one block) are not packed yet: every workgroup does it
@@ -604,9 +605,23 @@ mx4_product_kernel(const MxParams p) {
     auto finish = [&](int64_t tile) {
         const int64_t g = p.g0 + tile * p.gstep;
         if constexpr (MODE == MX_SCORES) {
+            const int c0 = (int)(p.row0 < 0 ? tile * TILE : g * 32 - p.row0);
+            if (p.past && (qb + 1) * BQ <= p.nq && c0 >= 0 && c0 + TILE <= p.n && !redo) {
+                char* o = (char*)p.out + ((size_t)qb * BQ * p.ld + c0) * 4;
+                const uint32_t at0 = (uint32_t)(4 * h * p.ld + l31) * 4;
+#pragma unroll
+                for (int c = 0; c < CG; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        char* line = o + (size_t)(c * 32 + (i & 3) + 8 * (i >> 2)) * p.ld * 4;
+#pragma unroll
+                        for (int r = 0; r < RG; ++r) __builtin_nontemporal_store(acc[r][c][i], (float*)(line + at0 + r * 128));
+                    }
+                return;
+            }
 #pragma unroll
             for (int r = 0; r < RG; ++r) {
-                const int64_t col = (p.row0 < 0 ? tile * TILE + r * 32 : (g + r) * 32 - p.row0) + l31;
+                const int col = c0 + r * 32 + l31;
                 if (col < 0 || col >= p.n) continue;
                 // (a row of the output at a time in scalar registers, the lane's column and its half of the rows as an offset)
                 const uint32_t at0 = (uint32_t)(4 * h * p.ld + col) * 4;

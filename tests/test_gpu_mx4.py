@@ -458,6 +458,25 @@ def test_scores_of_a_query_do_not_depend_on_the_others(R, torch):
             assert np.array_equal(ix.scores(tq[lo:lo + n]).cpu().numpy(), full[lo:lo + n], equal_nan=True)
 
 
+@pytest.mark.parametrize("nq,n,start", [(1030, 65600, 0), (1100, 65536, 32), (1100, 65536, 64), (1100, 65537, 0)])
+def test_scores_larger_than_the_caches(R, mx4, torch, nq, n, start):
+    """Those of 256 MB and more are stored another way where their lines are whole: the bits of smaller calls."""
+    ix = R.FlatIPIndex(200, storage="mx4")
+    g = torch.Generator(device="cuda").manual_seed(nq + n)
+    ix.add(torch.randn((n + 100, 200), generator=g, device="cuda"))
+    q = torch.randn((nq, 200), generator=g, device="cuda")
+    pair = mx4.quantize(q)
+    for whole, part in ((ix.scores(q, start, n), ix.scores(q, start + 1000, 30000)),
+                        (ix.scores_mx4(*pair, start, n), ix.scores_mx4(*pair, start + 1000, 30000))):
+        assert torch.equal(whole[:, 1000:31000], part)
+    few = mx4.quantize(q[-3:])
+    assert torch.equal(whole[-3:], ix.scores_mx4(*few, start, n))
+    q[5, 3] = float("inf")
+    big = ix.scores(q, start, n)
+    for lo, hi in ((0, 40), (40, 200)):
+        assert torch.allclose(big[lo:hi], ix.scores(q[lo:hi], start, n), rtol=0, atol=0, equal_nan=True)
+
+
 def test_scores_of_very_many_queries(R, mx4, torch):
     """More queries than one pass takes."""
     n = (1 << 18) + 70
