@@ -15,7 +15,9 @@
 // one scale. So a K-set is 64 elements (two blocks) and
 //   codes  [group of 32 rows][pair of K-sets][row][K-set of the pair][half][16 bytes]   (a last K-set without a partner:
 //          [row][half][16 bytes]): the two wave loads of a pair cover 2 KiB without a gap, and a single row is found in
-//          whole 64-byte pieces (rescoring and lookup gather rows; 32-byte pieces cost twice the traffic there)
+//          whole 64-byte pieces (rescoring and lookup gather rows; 32-byte pieces cost twice the traffic there. 128-byte ones, a
+//          quad of K-sets: 1000 queries x 500k rescored in 131 instead of 174 us, but scanned in 488 instead of 404: a tile's
+//          loads touch twice as many lines)
 //   scales [row][quad of 4 K-sets][half][4 bytes]   one dword = the scales of a lane's next four operands
 // Rows go from HBM straight into the registers of the one wave that multiplies them; LDS holds the queries only.
 //
