@@ -1462,11 +1462,12 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     constexpr int PARTS = MX_PARTS_SEARCH, FMT = ipx::MX_E2M3;
     const int64_t N = ix->ntotal;
     const int64_t groups = (N + ipx::MX_GROUP - 1) / ipx::MX_GROUP;
-    const bool timing = primary && ix->timing, direct = N <= ipx::MX_DIRECT;
+    const bool timing = primary && ix->timing;
     const int quad1 = PARTS * ipx::mx_part_bytes<FMT>(32);
     const MxGeom g = mx4_geometry(ix, nq, quad1, ipx::MX_SEARCH, groups);
     // The sample: more rows, hence a tighter floor and fewer hits, where the scores of the sample are few.
-    const int m_rows = nq <= 64 && N > 2 * ipx::MX_SAMPLE_FEW ? ipx::MX_SAMPLE_FEW : ipx::MX_SAMPLE_MANY;
+    const int m_room = nq <= 64 && N > 2 * ipx::MX_SAMPLE_FEW ? ipx::MX_SAMPLE_FEW : N >= ipx::MX_SAMPLE_MANY ? ipx::MX_SAMPLE_MANY : ipx::MX_SAMPLE_SHORT;
+    const int m_rows = (int)std::min<int64_t>(m_room, N);
     // j: the wanted list's share of the sample, plus 4 standard deviations of it and a little for short lists — the list
     // comes out too short (the query is then repeated) with a probability of about 1e-5.
     const double share = (double)kc * m_rows / (double)N;
@@ -1478,7 +1479,7 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     const int64_t waves = (int64_t)g.S * g.waves, nlists = 2 * waves;
     const int64_t tile_half = g.rg * ipx::MX_GROUP / 2, all = g.rounds * tile_half;
     const int64_t first_rows = ((int64_t)((hits + 64) / (2 * tile_half)) / waves + 1) * tile_half;
-    const int64_t want = direct ? all : std::min<int64_t>(all, std::max<int64_t>(first_rows, (int64_t)(1.5 * hits / nlists + 10.0 * sqrt(hits / nlists)) + 8));
+    const int64_t want = std::min<int64_t>(all, std::max<int64_t>(first_rows, (int64_t)(1.5 * hits / nlists + 10.0 * sqrt(hits / nlists)) + 8));
     const int64_t cap = std::min<int64_t>(want, (int64_t)0xffff0000u / (32 * g.cg * nlists * 8));      // (32-bit offsets in the kernel)
     const size_t info_bytes = ((size_t)nq * sizeof(ipx::MxQueryInfo) + 255) / 256 * 256, word = ((size_t)nq * 4 + 255) / 256 * 256;
 
@@ -1488,8 +1489,7 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     if (int rc = ix->candD.ensure((size_t)nq * kc * sizeof(float))) return rc;
     if (int rc = ix->candI.ensure((size_t)nq * kc * sizeof(int64_t))) return rc;
     if (int rc = ix->mxq.ensure(info_bytes + 3 * word)) return rc;         // norms, row bounds, floors, list states
-    if (!direct)
-        if (int rc = ix->mxs.ensure((size_t)nq * m_rows * sizeof(float))) return rc;
+    if (int rc = ix->mxs.ensure((size_t)nq * m_room * sizeof(float))) return rc;
     if (int rc = ensure_hflags(ix, nq, st)) return rc;
     ipx::MxQueryInfo* info = (ipx::MxQueryInfo*)ix->mxq.p;
     uint32_t* below = (uint32_t*)((char*)ix->mxq.p + info_bytes);
@@ -1498,8 +1498,7 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
 
     if (timing) IPX_HIP(hipEventRecord(ix->ev[0], st));
     hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)nq), dim3(256), 0, st, (const void*)qf,
-                       (int)IPX_F32, ix->d, PARTS, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, info, todo,
-                       direct ? tau : nullptr, below);
+                       (int)IPX_F32, ix->d, PARTS, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, info, todo);
     IPX_HIP(hipGetLastError());
     ipx::MxParams p = {};
     mx4_rows(ix, p);
@@ -1507,17 +1506,19 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     p.nq = (int)nq;
     p.q_dtype = IPX_F32;
     p.info = info;
-    if (!direct) {
+    {
         ipx::MxParams ps = p;
-        const MxGeom gs = mx4_geometry(ix, nq, quad1, ipx::MX_SCORES, m_rows / ipx::MX_GROUP);
-        ps.gstep = (N / ipx::MX_GROUP - gs.rg) / (gs.ntiles - 1);      // whole groups, spread over the index
+        const bool whole = m_rows == N;                                    // a short index: its rows in order
+        const MxGeom gs = mx4_geometry(ix, nq, quad1, ipx::MX_SCORES, whole ? groups : m_rows / ipx::MX_GROUP);
+        ps.gstep = whole ? gs.rg : (N / ipx::MX_GROUP - gs.rg) / (gs.ntiles - 1);      // whole groups, spread over the index
         ps.out = (float*)ix->mxs.p;
-        ps.ld = m_rows;
-        ps.row0 = -1;
+        ps.ld = m_room;
+        ps.row0 = whole ? 0 : -1;
         ps.n = m_rows;
         if (int rc = launch_mx4_product<PARTS, FMT, ipx::MX_SCORES>(gs, ps, st)) return rc;
-        hipLaunchKernelGGL((m_rows == ipx::MX_SAMPLE_FEW ? ipx::mx4_floor_kernel<ipx::MX_SAMPLE_FEW / 1024> : ipx::mx4_floor_kernel<ipx::MX_SAMPLE_MANY / 1024>),
-                           dim3((unsigned)nq), dim3(1024), 0, st, (const float*)ix->mxs.p, j, N, tau, below);
+        auto kern = m_room == ipx::MX_SAMPLE_FEW    ? ipx::mx4_floor_kernel<ipx::MX_SAMPLE_FEW / 1024>
+                    : m_room == ipx::MX_SAMPLE_MANY ? ipx::mx4_floor_kernel<ipx::MX_SAMPLE_MANY / 1024> : ipx::mx4_floor_kernel<ipx::MX_SAMPLE_SHORT / 1024>;
+        hipLaunchKernelGGL(kern, dim3((unsigned)nq), dim3(1024), 0, st, (const float*)ix->mxs.p, m_rows, j, N, tau, below);
         IPX_HIP(hipGetLastError());
     }
     if (timing) IPX_HIP(hipEventRecord(ix->ev[1], st));
@@ -1662,8 +1663,7 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
         // (the repeat pass has put other queries' norms where the rescoring kernel reads them)
         if (int rc = ix->Qp.ensure((size_t)((n + 31) / 32) * ix->nkq_x * ipx::mx_part_bytes<ipx::MX_E2M3>(32))) return rc;
         if (int rc = ix->mxq.ensure((size_t)n * sizeof(ipx::MxQueryInfo))) return rc;
-        hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)n), dim3(256), 0, st, (const void*)q, (int)IPX_F32, ix->d, 1, 32, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr,
-                       (float*)nullptr, (uint32_t*)nullptr);
+        hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)n), dim3(256), 0, st, (const void*)q, (int)IPX_F32, ix->d, 1, 32, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr);
         IPX_HIP(hipGetLastError());
         if (int rc = exact_rows_path(ix, q, hard, k, D, I, st)) return rc;
     }
@@ -1713,8 +1713,7 @@ int scores_slice(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sc
         if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
         if (int rc = ix->mxq.ensure((size_t)nq * sizeof(ipx::MxQueryInfo))) return rc;
         hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)nq), dim3(256), 0, st, dq, q_dtype, ix->d, MX_PARTS_SCORES,
-                           32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr, (float*)nullptr,
-                           (uint32_t*)nullptr);
+                           32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr);
         IPX_HIP(hipGetLastError());
         ix->Qp.captured |= captured;
         ix->mxq.captured |= captured;

@@ -39,7 +39,7 @@ constexpr int MX_KSET = 64;              // elements per K-set
 constexpr int MX_SET_BYTES = 1024;       // codes of one K-set of one group
 constexpr int MX_SAMPLE_FEW = 32768;     // rows a search samples for its floor: few queries (mx4_floor_kernel)
 constexpr int MX_SAMPLE_MANY = 8192;     // ... many
-constexpr int MX_DIRECT = 16384;         // indexes of up to this many rows are searched without a floor (fewer than the sample: neither)
+constexpr int MX_SAMPLE_SHORT = 4096;    // ... an index of fewer than 8192 rows (all of them below 4096)
 
 __device__ __forceinline__ float mx_scale_f32(uint32_t byte) {          // 2^(byte - 127); 255: NaN
     return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
@@ -361,11 +361,10 @@ __device__ __forceinline__ void mx_pack_lane(float (&x)[4], int b, int sub, int 
     }
 }
 
-// One workgroup per query. Eight lanes per block, four elements each. With `tau`, the
-// state of a search without a floor is written too: every row that scores a number is a hit.
+// One workgroup per query. Eight lanes per block, four elements each.
 __global__ void __launch_bounds__(256)
 mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int d, int parts, int bq, int nkq, uint8_t* __restrict__ dst,
-                        MxQueryInfo* __restrict__ info, int* __restrict__ todo, float* __restrict__ tau, uint32_t* __restrict__ row_below) {
+                        MxQueryInfo* __restrict__ info, int* __restrict__ todo) {
     __shared__ float red[8];
     const int tid = threadIdx.x, lane = tid & 63;
     bool nonzero = false;
@@ -393,10 +392,6 @@ mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int d, int part
     if (tid == 0) {
         info[q] = {red[0] + red[1] + red[2] + red[3] + least, red[4] + red[5] + red[6] + red[7] + least};
         if (todo) todo[q] = 0;
-        if (tau) {
-            tau[q] = -FLT_MAX;
-            row_below[q] = 0;
-        }
     }
 }
 
@@ -774,17 +769,35 @@ mx4_product_kernel(const MxParams p) {
     }
 }
 
+// Radix selection, one pass: the one of 256 counted values, highest first, that the need-th entry has, and how many entries with
+// it are wanted. At most one thread returns true and tells; none does when there are fewer than `need` entries. All threads of
+// the workgroup call it, between barriers; sums: 4 ints of LDS.
+__device__ __forceinline__ bool radix_pick(const int* counts, int need, int* sums, int& value, int& rest) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int c = tid < 256 ? counts[255 - tid] : 0;
+    int run = c;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const int y = __shfl_up(run, o); if (lane >= o) run += y; }
+    if (tid < 256 && lane == 63) sums[wave] = run;
+    __syncthreads();
+    if (tid >= 256) return false;
+    for (int w = 0; w < wave; ++w) run += sums[w];
+    value = 255 - tid;
+    rest = need - (run - c);
+    return run >= need && run - c < need;
+}
+
 // ---- the floor of a search -------------------------------------------------------------------------------------
 // A search scores a sample of the index first (whole tiles at equal distances) and takes about its j-th best score as the
 // floor every hit has to reach: with j well above the share of the wanted list that falls into the sample, about j / sample
 // of the index passes (the host chooses j: mx4_pass), which is a small multiple of the list.
-// One workgroup of 1024 per query, the sample's scores in registers. A histogram of 2047 steps of 2^-10 of a binade below
+// One workgroup of 1024 per query, the sample's scores in registers. A histogram of 2047 steps of 2^-9 of a binade below
 // the best score finds the step that the j-th lies in, and its lower edge is the floor. Where it lies lower, or in a step
 // with far more than j scores (equal scores), the j-th is found exactly by radix selection, and scores equal to it pass up
 // to a row: its share of the index, as equal scores are ordered by row.
 template <int PER>
 __global__ void __launch_bounds__(1024)
-mx4_floor_kernel(const float* __restrict__ sample, int j, int64_t N, float* __restrict__ tau, uint32_t* __restrict__ row_below) {
+mx4_floor_kernel(const float* __restrict__ sample, int m, int j, int64_t N, float* __restrict__ tau, uint32_t* __restrict__ row_below) {
     constexpr int M = PER * 1024;
     __shared__ int hist[2048];
     __shared__ uint32_t s_wave[16];
@@ -792,7 +805,7 @@ mx4_floor_kernel(const float* __restrict__ sample, int j, int64_t N, float* __re
     __shared__ int s_need, s_bin;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t q = blockIdx.x;
-    // entries 4 tid .. + 3 of every 4096: ordered score bits, 0 for what is never a hit (NaN, -inf)
+    // entries 4 tid .. + 3 of every 4096: ordered score bits, 0 for what is never a hit (NaN, -inf) and from entry m on
     uint32_t v[PER];
     uint32_t best = 0;
 #pragma unroll
@@ -801,7 +814,7 @@ mx4_floor_kernel(const float* __restrict__ sample, int j, int64_t N, float* __re
         const float s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            v[i + e] = s[e] > -FLT_MAX ? f32_ordered(s[e]) : 0u;
+            v[i + e] = s[e] > -FLT_MAX && i * 1024 + tid * 4 + e < m ? f32_ordered(s[e]) : 0u;
             best = max(best, v[i + e]);
         }
     }
@@ -816,7 +829,7 @@ mx4_floor_kernel(const float* __restrict__ sample, int j, int64_t N, float* __re
     for (int w = 0; w < 16; ++w) best = max(best, s_wave[w]);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const uint32_t bin = (best - v[i]) >> 13;
+        const uint32_t bin = (best - v[i]) >> 14;
         if (v[i] && bin < 2047) atomicAdd(&hist[bin], 1);
     }
     __syncthreads();
@@ -836,7 +849,7 @@ mx4_floor_kernel(const float* __restrict__ sample, int j, int64_t N, float* __re
     __syncthreads();
     if (s_bin >= 0) {
         if (tid == 0) {
-            const uint32_t steps = ((uint32_t)s_bin << 13) + 0x1fffu;       // the step's lowest score: this far below the best
+            const uint32_t steps = ((uint32_t)s_bin << 14) + 0x3fffu;       // the step's lowest score: this far below the best
             const uint32_t least = f32_ordered(-FLT_MAX) + 2;
             tau[q] = best >= least && best - least >= steps ? f32_below(f32_unordered(best - steps)) : -FLT_MAX;
             row_below[q] = 0;
@@ -852,21 +865,17 @@ mx4_floor_kernel(const float* __restrict__ sample, int j, int64_t N, float* __re
         for (int i = 0; i < PER; ++i)
             if (v[i] && (shift == 24 || (v[i] >> (shift + 8)) == (prefix >> (shift + 8)))) atomicAdd(&hist[(v[i] >> shift) & 255], 1);
         __syncthreads();
-        if (tid == 0) {
-            int b = 255, acc = 0;
-            while (b >= 0 && acc + hist[b] < s_need) acc += hist[b--];
-            if (b < 0) s_need = 0;                             // fewer than j numbers in the sample: no floor
-            else {
-                s_need -= acc;
-                s_prefix = prefix | (uint32_t)b << shift;
-            }
-        }
+        int value, rest;
+        const bool here = radix_pick(hist, s_need, (int*)s_wave, value, rest);
         __syncthreads();
-        if (s_need == 0) break;
+        if (here) { s_need = rest; s_prefix = prefix | (uint32_t)value << shift; }
+        if (here && shift == 24) s_bin = 0;
+        __syncthreads();
+        if (s_bin < 0) break;                                  // fewer than j numbers in the sample: no floor
     }
     const uint32_t t = s_prefix;
     const int need = s_need;                                   // the need-th of the entries equal to t, in row order
-    if (need == 0) {
+    if (s_bin < 0) {
         if (tid == 0) { tau[q] = -FLT_MAX; row_below[q] = 0; }
         return;
     }
@@ -891,7 +900,7 @@ mx4_floor_kernel(const float* __restrict__ sample, int j, int64_t N, float* __re
         for (int e = 0; e < 4; ++e)
             if ((eq >> e & 1) && ++k == need) {
                 tau[q] = f32_unordered(t);
-                const int64_t rows = ((int64_t)(i * 1024 + tid * 4 + e + 1) * N + M - 1) / M;
+                const int64_t rows = ((int64_t)(i * 1024 + tid * 4 + e + 1) * N + m - 1) / m;
                 row_below[q] = (uint32_t)((rows + 31) / 32 * 32);
             }
         done += total;
@@ -1017,12 +1026,10 @@ mx4_select_kernel(const uint2* __restrict__ lists, const int* __restrict__ cnt, 
                 if (sh == 56 || (key >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[(int)(key >> sh) & 255], 1);
             });
             __syncthreads();
-            if (tid == 0) {
-                int b = 255, acc = 0;
-                while (b > 0 && acc + hist[b] < s_need) acc += hist[b--];
-                s_need -= acc;
-                s_prefix = prefix | (uint64_t)b << sh;
-            }
+            int value, rest;
+            const bool here = radix_pick(hist, s_need, s_sum, value, rest);
+            __syncthreads();
+            if (here) { s_need = rest; s_prefix = prefix | (uint64_t)value << sh; }
         }
         __syncthreads();
         const uint64_t kth = s_prefix;                         // keys are distinct: kc of them reach it
