@@ -18,8 +18,8 @@
  *     without synchronising. With a bf16 copy or 4-bit rows (storage 1, 2, 3) ipx_search /
  *     ipx_search_aspect / ipx_search_pooled read back one flag word per query
  *     after the rescoring pass (which queries the margin rule sends to a repeat
- *     pass) and so synchronise the stream once per pass before they return (storage 3: not on an index of up to 4096
- *     rows with nq * rows <= 2^20, which takes one launch);
+ *     pass) and so synchronise the stream once per pass before they return (storage 3: not where
+ *     the index is so short that every row is scored in one launch: 1000 rows of 768, up to 1000 queries);
  *     ipx_merge_topk synchronises when a list exceeds IPX_MAX_K entries.
  *   - an index serves one call at a time: its scratch buffers, timing events
  *     and last-search statistics are per index, not per call. Concurrent

@@ -815,7 +815,8 @@ int launch_rescore(const ipx::RescoreParams& rp, int64_t nblocks, hipStream_t st
     const int fixed = ((dpad * 4 + 15) & ~15) + rp.P * 8 + (rp.P <= ipx::RS_RANK_SORT || rp.xfmt == 2 ? rp.P * 8 : 0);
     if (rp.xfmt == 2) {
         const int per_wave = 64 * ipx::RS_ROW;
-        const bool few = nblocks <= 128 && fixed + 16 * per_wave <= 160 * 1024;
+        // (16 waves: a workgroup alone on its CU. Scoring every row, there are enough rows for them: 256 queries x 4000 rows)
+        const bool few = nblocks <= (rp.all_rows ? 256 : 128) && fixed + 16 * per_wave <= 160 * 1024;
         const int lds = fixed + (few ? 16 : 4) * per_wave;
         void (*kern)(const ipx::RescoreParams) = few ? ipx::rescore_kernel<16, true> : ipx::rescore_kernel<4, true>;
         if (int rc = ensure_dynamic_lds((const void*)kern, lds)) return rc;
@@ -1390,7 +1391,14 @@ constexpr int MX_PACK_HERE = 4;
 constexpr int64_t MX_SCORES_SLICE = 1 << 18;      // queries per pass of ipx_scores: bounds the workspace (4 KB a query of 768) and a launch's threads
 constexpr int MX_MAX_K = IPX_MAX_K;      // deepest list of a search
 constexpr int MX_SLICE = 4096;           // queries per pass of a search (bounds the workspace)
-constexpr int64_t MX_WHOLE = 4096, MX_WHOLE_PAIRS = 1 << 20;      // scan_mx4_path: rows, rows x queries scored without a scan
+// A short index and not many queries: the exact score of every row at once, one launch and nothing to prove (and no
+// synchronisation). That takes one CU per query about as long as the rows' elements and, at 384 elements a row, their sorting;
+// the passes take 45-90 us whatever the rows. Every row -> passes, us: 1 query of 768: 1000 rows 22 -> 53, 2000 41 -> 52, 3000
+// 58 -> 52; of 128: 4000 44 -> 45; 500 queries of 768: 1000 rows 50 -> 74, 1500 76 -> 74; of 128: 2000 53 -> 62, 3000 86 -> 57.
+bool mx4_score_every_row(int64_t rows, int64_t nq, int d) {
+    const int64_t work = rows * (d + 384);
+    return nq <= 256 ? rows <= 4096 && work <= 2600000 : rows <= 2048 && rows * nq <= 1 << 20 && work <= 1600000;
+}
 
 // How a product runs: 32-query groups per workgroup (cg), splits of the corpus, whether the query block stays in LDS; the
 // row groups of a wave tile and the waves of a workgroup.
@@ -1595,10 +1603,7 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
     // The list has to reach e below the k-th score (rescore_kernel, post): 1.8M Gaussian rows of 768, k = 100: 120 left 2 of
     // 64 queries to the repeat pass, 125 none; 500k, k = 1000: 1100 left 131 of 1000, 1150 none. Rows whose norms spread
     // widen e: the list then grows as in the bf16 scan (ipx_index::kc_boost).
-    // A short index and not many queries: the exact score of every row at once, one launch and nothing to prove (and no
-    // synchronisation). 3 queries, 999 rows of 100: 43 us for the passes below. The limit: 16 chains of 64 rows keep a CU busy for about
-    // as long as the passes take.
-    if (ix->ntotal <= MX_WHOLE && nq * ix->ntotal <= MX_WHOLE_PAIRS && ix->force_kc == 0) {
+    if (mx4_score_every_row(ix->ntotal, nq, ix->d) && ix->force_kc == 0) {
         ipx::RescoreParams rp;
         rp.candD = nullptr;
         rp.candI = nullptr;
