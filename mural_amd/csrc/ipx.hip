@@ -351,24 +351,22 @@ int lookup_lanes(int np) {
 }
 // A launch numbers its threads with 32 bits: rows per launch when a row takes `per_row` of them.
 int64_t rows_per_launch(int64_t per_row) { return std::max<int64_t>(1, (int64_t)(1ll << 31) / per_row); }
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Rows (device, `stride` elements apart) -> mx4: codes / scales in the external form, or rows row0.. of index ix.
 int launch_mx4_quantize(const void* rows, int dtype, int64_t n, int d, int64_t stride, uint8_t* codes, uint8_t* scales,
                         ipx_index* ix, int64_t row0, hipStream_t st) {
     const int nb = (d + 31) / 32, np = nb * 4;
     const size_t el = dtype == IPX_F32 ? 4 : 2;
-    const bool wide = aligned16(rows) && stride * el % 16 == 0;
     const int64_t slice = rows_per_launch(np);
     for (int64_t r0 = 0; r0 < n; r0 += slice) {
         const uint32_t total = (uint32_t)(std::min(slice, n - r0) * np);
         const void* src = (const char*)rows + (size_t)r0 * stride * el;
         const dim3 grid((total + 255) / 256), block(256);
         if (ix)
-            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<true>, grid, block, 0, st, src, dtype, stride, total, magic_of(np), np, d, wide,
+            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<true>, grid, block, 0, st, src, dtype, stride, total, magic_of(np), np, d,
                                ix->Xx, ix->Xxs, row0 + r0, ix->nks_x, ix->nkq_x);
         else
-            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<false>, grid, block, 0, st, src, dtype, stride, total, magic_of(np), np, d, wide,
+            hipLaunchKernelGGL(ipx::mx4_quantize_kernel<false>, grid, block, 0, st, src, dtype, stride, total, magic_of(np), np, d,
                                codes + (size_t)r0 * nb * 16, scales + (size_t)r0 * nb, (int64_t)0, 0, 0);
         IPX_HIP(hipGetLastError());
     }
@@ -2185,7 +2183,6 @@ int ipx_lookup(ipx_index* ix, const int64_t* ids, int64_t n, const float* scale,
     const int xfmt = ix->storage == 3 ? 2 : ix->storage == 2 ? 1 : 0;
     const void* X = xfmt == 2 ? (const void*)ix->Xx : xfmt ? (const void*)ix->Xh : (const void*)ix->Xp;
     const int nks = xfmt == 2 ? ix->nks_x : xfmt ? ix->nks_h : ix->nks;
-    const bool wide = aligned16(dout) && row_bytes % 16 == 0;
     const int l2 = lookup_lanes(np);
     const int64_t slice = rows_per_launch(1 << l2);
     auto kern = xfmt == 2 ? ipx::lookup_kernel<2> : xfmt == 1 ? ipx::lookup_kernel<1> : ipx::lookup_kernel<0>;
@@ -2193,7 +2190,7 @@ int ipx_lookup(ipx_index* ix, const int64_t* ids, int64_t n, const float* scale,
         const uint32_t m = (uint32_t)std::min(slice, n - i0);
         hipLaunchKernelGGL(kern, dim3((unsigned)((((int64_t)m << l2) + 255) / 256)), dim3(256), 0, st, X, (const uint8_t*)ix->Xxs, nks,
                            ix->nkq_x, ix->id_base, ix->ntotal, di + i0, ds ? ds + i0 : nullptr, m, l2, np, d,
-                           (void*)(dout + (size_t)i0 * row_bytes), dtype, wide, (int*)ix->err.p + LOOKUP_ERR);
+                           (void*)(dout + (size_t)i0 * row_bytes), dtype, (int*)ix->err.p + LOOKUP_ERR);
         IPX_HIP(hipGetLastError());
     }
     if (!on_device) {
@@ -2260,13 +2257,11 @@ int ipx_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n, i
         dout = (char*)o.p;
     }
     const int np = (d + 7) / 8;
-    // (the wide form also reads the codes as dwords: they then start at a multiple of 4 bytes)
-    const bool wide = aligned16(dout) && row_bytes % 16 == 0 && ((uintptr_t)dc & 3) == 0;
     const int64_t slice = rows_per_launch(np);
     for (int64_t r0 = 0; r0 < n && e == hipSuccess; r0 += slice) {
         const uint32_t total = (uint32_t)(std::min(slice, n - r0) * np);
         hipLaunchKernelGGL(ipx::mx4_dequantize_kernel, dim3((total + 255) / 256), dim3(256), 0, st, dc + (size_t)r0 * nb * 16,
-                           ds + (size_t)r0 * nb, total, magic_of(np), np, d, (int)nb, (void*)(dout + (size_t)r0 * row_bytes), dtype, wide);
+                           ds + (size_t)r0 * nb, total, magic_of(np), np, d, (int)nb, (void*)(dout + (size_t)r0 * row_bytes), dtype);
         e = hipGetLastError();
     }
     if (!on_device) {

@@ -86,16 +86,22 @@ __device__ __forceinline__ uint32_t pack2_as(int dtype, float lo, float hi) {   
     if (dtype == 1) return __builtin_bit_cast(uint32_t, f16x2{(_Float16)lo, (_Float16)hi});
     return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
 }
-// `count` of eight outputs from element i on; `wide`: they start at a multiple of 16 bytes
-__device__ __forceinline__ void store8(void* out, int dtype, size_t i, const float (&v)[8], int count, bool wide) {
-    if (wide && count >= 8) {
+// Callers' rows and codes start where they like (rows of 767 elements, a slice): the memory takes 16 bytes from any address, so
+// they are read and written whole all the same. (One element at a time, rows of 767 went at 1.9-2.6 TB/s, those of 768 at 5.0-5.8.)
+typedef uint32_t any_u32 __attribute__((aligned(1)));
+typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// `count` of eight outputs from element i on
+__device__ __forceinline__ void store8(void* out, int dtype, size_t i, const float (&v)[8], int count) {
+    if (count >= 8) {
         if (dtype == 0) {
-            float4* o = (float4*)((float*)out + i);
-            o[0] = make_float4(v[0], v[1], v[2], v[3]);
-            o[1] = make_float4(v[4], v[5], v[6], v[7]);
+            float* o = (float*)out + i;
+            *(f32x4_at4*)o = f32x4_at4{v[0], v[1], v[2], v[3]};
+            *(f32x4_at4*)(o + 4) = f32x4_at4{v[4], v[5], v[6], v[7]};
         } else {
-            *(uint4*)((uint16_t*)out + i) = make_uint4(pack2_as(dtype, v[0], v[1]), pack2_as(dtype, v[2], v[3]),
-                                                       pack2_as(dtype, v[4], v[5]), pack2_as(dtype, v[6], v[7]));
+            *(u32x4_at2*)((uint16_t*)out + i) = u32x4_at2{pack2_as(dtype, v[0], v[1]), pack2_as(dtype, v[2], v[3]),
+                                                          pack2_as(dtype, v[4], v[5]), pack2_as(dtype, v[6], v[7])};
         }
         return;
     }
@@ -119,7 +125,7 @@ __device__ __forceinline__ uint32_t div_by(uint32_t i, uint64_t magic) {      //
 // lanes away. Bound by HBM.
 template <bool INDEX>
 __global__ void __launch_bounds__(256)
-mx4_quantize_kernel(const void* __restrict__ src, int dtype, int64_t stride, uint32_t total, uint64_t magic, int np, int d, bool wide,
+mx4_quantize_kernel(const void* __restrict__ src, int dtype, int64_t stride, uint32_t total, uint64_t magic, int np, int d,
                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t row0, int nks, int nkq) {
     const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
     if (gid >= total) return;                               // a multiple of 4: the four lanes of a block stay together
@@ -129,17 +135,16 @@ mx4_quantize_kernel(const void* __restrict__ src, int dtype, int64_t stride, uin
         const int e0 = piece * 8;
         const int64_t at = (int64_t)r * stride + e0;
         float x[8];
-        if (wide && e0 + 8 <= d) {
+        if (e0 + 8 <= d) {
             if (dtype == 0) {
-                const float4 a = *(const float4*)((const float*)src + at), b = *(const float4*)((const float*)src + at + 4);
-                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                const f32x4 a = *(const f32x4_at4*)((const float*)src + at), b = *(const f32x4_at4*)((const float*)src + at + 4);
+                x[0] = a[0]; x[1] = a[1]; x[2] = a[2]; x[3] = a[3]; x[4] = b[0]; x[5] = b[1]; x[6] = b[2]; x[7] = b[3];
             } else {
-                const uint4 w = *(const uint4*)((const uint16_t*)src + at);
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                const u32x4_at2 ws = *(const u32x4_at2*)((const uint16_t*)src + at);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (dtype == 1) {
-                        const f16x2 v = __builtin_bit_cast(f16x2, ws[e]);
+                        const f16x2 v = __builtin_bit_cast(f16x2, (uint32_t)ws[e]);
                         x[2 * e] = (float)v[0];
                         x[2 * e + 1] = (float)v[1];
                     } else {
@@ -182,8 +187,7 @@ mx4_place_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ 
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint8_t* s = codes + (size_t)gid * 16 + 4 * i;            // (the caller's bytes may start anywhere)
-        w[i] = s[0] | (uint32_t)s[1] << 8 | (uint32_t)s[2] << 16 | (uint32_t)s[3] << 24;
+        w[i] = *(const any_u32*)(codes + (size_t)gid * 16 + 4 * i);
         const int left = d - b * 32 - i * 8;                            // codes behind element d count as 0
         if (left < 8) w[i] &= left <= 0 ? 0u : (1u << (4 * left)) - 1u;
     }
@@ -194,17 +198,16 @@ mx4_place_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ 
 // external form -> values
 __global__ void __launch_bounds__(256)
 mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t total, uint64_t magic, int np,
-                      int d, int nb, void* __restrict__ out, int dtype, bool wide) {
+                      int d, int nb, void* __restrict__ out, int dtype) {
     const uint32_t gid = blockIdx.x * 256u + threadIdx.x;
     if (gid >= total) return;
     const uint32_t r = np == 1 ? gid : div_by(gid, magic);
     const int piece = (int)(gid - r * (uint32_t)np);
     const size_t blk = (size_t)r * nb + (piece >> 2);
-    const uint8_t* s = codes + blk * 16 + (piece & 3) * 4;
-    const uint32_t w = wide ? *(const uint32_t*)s : s[0] | (uint32_t)s[1] << 8 | (uint32_t)s[2] << 16 | (uint32_t)s[3] << 24;
+    const uint32_t w = *(const any_u32*)(codes + blk * 16 + (piece & 3) * 4);
     float v[8];
     mx_decode8(w, scales[blk], v);
-    store8(out, dtype, (size_t)r * d + piece * 8, v, d - piece * 8, wide);
+    store8(out, dtype, (size_t)r * d + piece * 8, v, d - piece * 8);
 }
 
 // max |x|^2 over rows [row0, row0 + n) of an mx4 index, for the margin rule (rescore_kernel), as float bits. A row with a
@@ -251,7 +254,7 @@ template <int XFMT>
 __global__ void __launch_bounds__(256)
 lookup_kernel(const void* __restrict__ X, const uint8_t* __restrict__ Xs, int nks, int nkq, int64_t id_base, int64_t N,
               const int64_t* __restrict__ ids, const float* __restrict__ scale, uint32_t n, int l2, int np, int d,
-              void* __restrict__ out, int dtype, bool wide, int* err) {
+              void* __restrict__ out, int dtype, int* err) {
     constexpr int AHEAD = 4;                                   // pieces a lane has in flight
     const uint32_t gid = blockIdx.x * 256u + threadIdx.x, i = gid >> l2;
     if (i >= n) return;
@@ -301,7 +304,7 @@ lookup_kernel(const void* __restrict__ X, const uint8_t* __restrict__ Xs, int nk
             if (scale && have)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= s;
-            store8(out, dtype, (size_t)i * d + piece * 8, v, d - piece * 8, wide);
+            store8(out, dtype, (size_t)i * d + piece * 8, v, d - piece * 8);
         }
     }
 }
@@ -408,8 +411,7 @@ mx4_pack_codes_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
     if (b < nb) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint8_t* s = codes + ((size_t)q * nb + b) * 16 + 4 * i;
-            w[i] = s[0] | (uint32_t)s[1] << 8 | (uint32_t)s[2] << 16 | (uint32_t)s[3] << 24;
+            w[i] = *(const any_u32*)(codes + ((size_t)q * nb + b) * 16 + 4 * i);
             const int left = d - b * 32 - i * 8;
             if (left < 8) w[i] &= left <= 0 ? 0u : (1u << (4 * left)) - 1u;
         }
