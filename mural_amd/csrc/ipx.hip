@@ -1380,8 +1380,8 @@ int scan_bf16_path(ipx_index* ix, const float* dq, const float* dw, int A, int l
 }
 
 // ---- mx4 rows (storage 3) -------------------------------------------------------------------------------------
-constexpr int MX_PARTS_SEARCH = 2;       // E2M3 parts per query in the scan: what they leave out enters the margin rule
-constexpr int MX_PARTS_SCORES = 5;       // ... in ipx_scores: as exact as fp32
+using ipx::MX_PARTS_SCORES;
+using ipx::MX_PARTS_SEARCH;
 // ipx_scores: up to this many queries are packed by the product kernel itself, in every workgroup, not by a kernel before it
 // (with it -> without, us; 1 query: 1000 x 768 rows 13.9 -> 9.4, 100k 17.3 -> 15.0, 1M 90 -> 91; 4 queries: 13.8 -> 10.9,
 // 17.3 -> 16.1, 97 -> 96.5; 8 queries: 13.9 -> 12.9, 17.9 -> 18.3, 103 -> 108)
@@ -1461,6 +1461,16 @@ void mx4_rows(const ipx_index* ix, ipx::MxParams& p) {
 // magnitudes, at most |q||x|) to the running sum (2^-24 of it each time). Taken 4x, as there.
 float mx4_acc_coef(int d, int nks, int parts) { return (float)((d + 1 + 4.0 * (nks * parts + 64)) / 16777216.0 * 1.002); }
 
+// fp32 (f16, bf16) queries -> parts, their norms, `todo` cleared
+int launch_mx4_pack(ipx_index* ix, const void* q, int dtype, int64_t nq, int parts, int bq, ipx::MxQueryInfo* info, int* todo, hipStream_t st) {
+    int l2 = 3;
+    while (l2 < 6 && (1 << l2) < ix->nkq_x * 8) ++l2;
+    hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)(((nq << l2) + 255) / 256)), dim3(256), 0, st, q, dtype, (int)nq, ix->d, parts,
+                       bq, ix->nkq_x, l2, (uint8_t*)ix->Qp.p, info, todo);
+    IPX_HIP(hipGetLastError());
+    return 0;
+}
+
 // One search pass over the 4-bit rows: pack -> floor (from a sample) -> scan -> the kc best hits -> exact rescoring.
 // The contract of bf16_pass.
 int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* dD, int64_t* dI, hipStream_t st, bool primary,
@@ -1503,9 +1513,7 @@ int mx4_pass(ipx_index* ix, const float* qf, int64_t nq, int k, int kc, float* d
     int* todo = (int*)((char*)ix->mxq.p + info_bytes + 2 * word);
 
     if (timing) IPX_HIP(hipEventRecord(ix->ev[0], st));
-    hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)nq), dim3(256), 0, st, (const void*)qf,
-                       (int)IPX_F32, ix->d, PARTS, 32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, info, todo);
-    IPX_HIP(hipGetLastError());
+    if (int rc = launch_mx4_pack(ix, qf, IPX_F32, nq, PARTS, 32 * g.cg, info, todo, st)) return rc;
     ipx::MxParams p = {};
     mx4_rows(ix, p);
     p.Q = (const uint8_t*)ix->Qp.p;
@@ -1666,8 +1674,7 @@ int scan_mx4_path(ipx_index* ix, const float* dq, const float* dw, int A, int lo
         // (the repeat pass has put other queries' norms where the rescoring kernel reads them)
         if (int rc = ix->Qp.ensure((size_t)((n + 31) / 32) * ix->nkq_x * ipx::mx_part_bytes<ipx::MX_E2M3>(32))) return rc;
         if (int rc = ix->mxq.ensure((size_t)n * sizeof(ipx::MxQueryInfo))) return rc;
-        hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)n), dim3(256), 0, st, (const void*)q, (int)IPX_F32, ix->d, 1, 32, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr);
-        IPX_HIP(hipGetLastError());
+        if (int rc = launch_mx4_pack(ix, q, IPX_F32, n, 1, 32, (ipx::MxQueryInfo*)ix->mxq.p, nullptr, st)) return rc;
         if (int rc = exact_rows_path(ix, q, hard, k, D, I, st)) return rc;
     }
     return 0;
@@ -1715,9 +1722,7 @@ int scores_slice(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sc
     if (!p.pack_here) {
         if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
         if (int rc = ix->mxq.ensure((size_t)nq * sizeof(ipx::MxQueryInfo))) return rc;
-        hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)nq), dim3(256), 0, st, dq, q_dtype, ix->d, MX_PARTS_SCORES,
-                           32 * g.cg, ix->nkq_x, (uint8_t*)ix->Qp.p, (ipx::MxQueryInfo*)ix->mxq.p, (int*)nullptr);
-        IPX_HIP(hipGetLastError());
+        if (int rc = launch_mx4_pack(ix, dq, q_dtype, nq, MX_PARTS_SCORES, 32 * g.cg, (ipx::MxQueryInfo*)ix->mxq.p, nullptr, st)) return rc;
         ix->Qp.captured |= captured;
         ix->mxq.captured |= captured;
         p.Q = (const uint8_t*)ix->Qp.p;

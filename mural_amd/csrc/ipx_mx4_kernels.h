@@ -319,81 +319,112 @@ constexpr int MX_E2M3 = 2, MX_E2M1 = 4;      // operand format numbers of the in
 template <int FMT> __host__ __device__ constexpr int mx_code_bytes() { return FMT == MX_E2M3 ? 24 : 16; }
 template <int FMT> __host__ __device__ constexpr int mx_part_bytes(int bq) { return bq * (8 * mx_code_bytes<FMT>() + 8); }
 
+constexpr int MX_PARTS_SEARCH = 2;       // E2M3 parts per query in the scan: what they leave out enters the margin rule
+constexpr int MX_PARTS_SCORES = 5;       // ... in ipx_scores: as exact as fp32
 struct MxQueryInfo {      // of one query
     float sumsq;          // |q|^2                          (both 1e-37 larger where q has a nonzero element: squares of
     float restsq;         // |q - sum of its parts|^2        very small elements vanish, the bounds they stand for must not)
 };
 
-// One lane's four elements of block b (K-set b >> 1, half b & 1) of query ql into its block; the eight lanes of a block are
-// neighbours, `sub` is the lane's number among them. x: the elements, then what the parts leave (0 in a block
-// with a NaN or an infinity, whose scales are NaN).
-__device__ __forceinline__ void mx_pack_lane(float (&x)[4], int b, int sub, int parts, int bq, int ql, uint8_t* block) {
-    const int part_bytes = bq * 200, quad = b >> 3, j = (b >> 1) & 3, h = b & 1;
-    bool bad = false;
-    for (int p = 0; p < parts; ++p) {
+typedef float f32x32 __attribute__((ext_vector_type(32)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+// A block of 32 elements, the even ones and the odd ones apart as the conversion to E2M3 takes them.
+struct MxBlock { f32x16 even, odd; };
+
+__device__ __forceinline__ MxBlock mx_load_block(const void* src, int dtype, int64_t at, int left) {      // left: elements there are
+    MxBlock x;
+    if (left >= 32) {
+        if (dtype == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const f32x4 v = *(const f32x4_at4*)((const float*)src + at + 4 * i);
+                x.even[2 * i] = v[0]; x.odd[2 * i] = v[1]; x.even[2 * i + 1] = v[2]; x.odd[2 * i + 1] = v[3];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u32x4_at2 w = *(const u32x4_at2*)((const uint16_t*)src + at + 8 * i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f16x2 v = __builtin_bit_cast(f16x2, (uint32_t)w[e]);
+                    x.even[4 * i + e] = dtype == 1 ? (float)v[0] : bf16_lo(w[e]);
+                    x.odd[4 * i + e] = dtype == 1 ? (float)v[1] : bf16_hi(w[e]);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x.even[i] = 2 * i < left ? load_as_f32(src, dtype, at + 2 * i) : 0.f;
+            x.odd[i] = 2 * i + 1 < left ? load_as_f32(src, dtype, at + 2 * i + 1) : 0.f;
+        }
+    }
+    return x;
+}
+
+// One lane: block b (K-set b >> 1, half b & 1) of query ql into its query block. x: the elements, then what the parts leave (0 in a
+// block with a NaN or an infinity, whose scales are NaN). Codes are rounded to nearest even by the conversion, and what it
+// made of them is taken off again, so that nothing here depends on how it rounds.
+__device__ __forceinline__ void mx_pack_block(MxBlock& x, int b, int parts, int bq, int ql, uint8_t* block) {
+    const int quad = b >> 3, j = (b >> 1) & 3, h = b & 1, place = (j * 2 + h) * bq + ql;
+    uint8_t* part = block + (size_t)quad * parts * bq * 200;
+#pragma unroll 1
+    for (int p = 0; p < parts; ++p, part += bq * 200) {
         uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-        top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, true));       // quad_perm [1,0,3,2]
-        top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true));       // quad_perm [2,3,0,1]
-        top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xF, 0xF, true));      // row_half_mirror
-        bad |= top >= 0x7f800000u;                                  // NaN / inf: the block's scales are NaN
-        // smallest s in [-127, 125] with the largest magnitude <= 7.5 x 2^s
-        const int s = max((int)(top >> 23) - 129 + ((top & 0x7fffffu) > 0x700000u ? 1 : 0), -127);
-        const float inv = __uint_as_float((uint32_t)(127 - s) << 23), scale = mx_scale_f32((uint32_t)(s + 127));
-        uint32_t bits = 0;
+        for (int e = 0; e < 16; ++e) top = max(top, max(__float_as_uint(x.even[e]) & 0x7fffffffu, __float_as_uint(x.odd[e]) & 0x7fffffffu));
+        const bool bad = top >= 0x7f800000u;
+        // smallest s in [-127, 126] with the largest magnitude <= 7.5 x 2^s
+        const uint32_t byte = (uint32_t)max((int)(top >> 23) - 2 + ((top & 0x7fffffu) > 0x700000u ? 1 : 0), 0);
+        const float scale = mx_scale_field(byte);
+        u32x6 c = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(x.even, x.odd, scale);
+        const f32x32 v = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(c, scale);
+        // (hipcc lets the result of either conversion share registers with its last operands, which it then overwrites before
+        // they are read: kept in use until here, they cannot be shared)
+        asm volatile("" ::"v"(x.even), "v"(x.odd), "v"(scale), "v"(c));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (bad) { x[e] = 0.f; continue; }
-            const float a = fabsf(x[e]) * inv;
-            // codes count steps of 1/8 below 2, 1/4 below 4, 1/2 up to 7.5
-            const float per = a < 2.f ? 8.f : a < 4.f ? 4.f : 2.f, step = a < 2.f ? 0.125f : a < 4.f ? 0.25f : 0.5f;
-            const float c = rintf(a * per), v = c * step;
-            const uint32_t neg = __float_as_uint(x[e]) >> 31, code = (uint32_t)((int)c + (a < 2.f ? 0 : a < 4.f ? 8 : 16));
-            bits |= (code | neg << 5) << (6 * e);
-            x[e] -= (neg ? -v : v) * scale;                         // exact: both are multiples of x's last place
+        for (int e = 0; e < 16; ++e) {
+            x.even[e] = bad ? 0.f : x.even[e] - v[2 * e];           // exact: both are multiples of x's last place
+            x.odd[e] = bad ? 0.f : x.odd[e] - v[2 * e + 1];
         }
-        uint8_t* part = block + ((size_t)quad * parts + p) * part_bytes;
-        // the lane's 24 bits are bytes 3 sub .. 3 sub + 2 of the block's 24
-#pragma unroll
-        for (int y = 0; y < 3; ++y) {
-            const int at = sub * 3 + y;
-            part[at < 16 ? ((j * 2 + h) * bq + ql) * 16 + at : bq * 128 + ((j * 2 + h) * bq + ql) * 8 + (at - 16)] = (uint8_t)(bits >> (8 * y));
-        }
-        if (sub == 0) part[bq * 192 + (h * bq + ql) * 4 + j] = bad ? 255 : (uint8_t)(s + 127);
+        if (bad) c = u32x6{};
+        *(uint4*)(part + place * 16) = make_uint4(c[0], c[1], c[2], c[3]);
+        *(uint2*)(part + bq * 128 + place * 8) = make_uint2(c[4], c[5]);
+        part[bq * 192 + (h * bq + ql) * 4 + j] = bad ? 255 : (uint8_t)byte;
     }
 }
 
-// One workgroup per query. Eight lanes per block, four elements each.
+// A lane per block; 2^l2 lanes (8 to 64) per query. Neighbouring queries write neighbouring 16-byte pieces: they share a
+// workgroup, and an XCD. 3813 queries of 576 in 5 parts: 17 us; four elements a lane,
+// converted by ordinary arithmetic, took 24.
 __global__ void __launch_bounds__(256)
-mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int d, int parts, int bq, int nkq, uint8_t* __restrict__ dst,
-                        MxQueryInfo* __restrict__ info, int* __restrict__ todo) {
-    __shared__ float red[8];
-    const int tid = threadIdx.x, lane = tid & 63;
-    bool nonzero = false;
-    const int64_t q = blockIdx.x;
+mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, int parts, int bq, int nkq, int l2,
+                        uint8_t* __restrict__ dst, MxQueryInfo* __restrict__ info, int* __restrict__ todo) {
+    const int64_t q = ((int64_t)xcd_remap(blockIdx.x, gridDim.x) * 256 + threadIdx.x) >> l2;
+    if (q >= nq) return;
     uint8_t* block = dst + (size_t)(q / bq) * nkq * parts * bq * 200;
-    const int ql = (int)(q % bq), sub = tid & 7;
+    const int lanes = 1 << l2, first = threadIdx.x & (lanes - 1), ql = (int)(q % bq);
+    int nonzero = 0;
     float ss = 0.f, rr = 0.f;
-    for (int b = tid >> 3; b < nkq * 8; b += 32) {
-        float x[4];
+    for (int b = first; b < nkq * 8; b += lanes) {
+        MxBlock x = mx_load_block(src, dtype, q * (int64_t)d + b * 32, d - b * 32);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int at = b * 32 + sub * 4 + e;
-            x[e] = at < d ? load_as_f32(src, dtype, q * (int64_t)d + at) : 0.f;
-            ss = fmaf(x[e], x[e], ss);
-            nonzero |= x[e] != 0.f;
+        for (int e = 0; e < 16; ++e) {
+            ss = fmaf(x.even[e], x.even[e], fmaf(x.odd[e], x.odd[e], ss));
+            nonzero |= x.even[e] != 0.f || x.odd[e] != 0.f;
         }
-        mx_pack_lane(x, b, sub, parts, bq, ql, block);
+        mx_pack_block(x, b, parts, bq, ql, block);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) rr = fmaf(x[e], x[e], rr);
+        for (int e = 0; e < 16; ++e) rr = fmaf(x.even[e], x.even[e], fmaf(x.odd[e], x.odd[e], rr));
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) { ss += __shfl_xor(ss, off); rr += __shfl_xor(rr, off); }
-    if (lane == 0) { red[tid >> 6] = ss; red[4 + (tid >> 6)] = rr; }
-    const float least = __syncthreads_or(nonzero) ? 1e-37f : 0.f;
-    if (tid == 0) {
-        info[q] = {red[0] + red[1] + red[2] + red[3] + least, red[4] + red[5] + red[6] + red[7] + least};
+    for (int off = lanes >> 1; off > 0; off >>= 1) {
+        ss += __shfl_xor(ss, off);
+        rr += __shfl_xor(rr, off);
+        nonzero |= __shfl_xor(nonzero, off);
+    }
+    if (first == 0) {
+        const float least = nonzero ? 1e-37f : 0.f;
+        info[q] = {ss + least, rr + least};
         if (todo) todo[q] = 0;
     }
 }
@@ -490,6 +521,7 @@ __global__ void __launch_bounds__(WAVES * 64)
 mx4_product_kernel(const MxParams p) {
     constexpr int BQ = 32 * CG, PART = mx_part_bytes<FMT>(BQ), QUAD = PARTS * PART, CODES = mx_code_bytes<FMT>();
     constexpr int TILE = RG * MX_GROUP, THREADS = WAVES * 64;
+    constexpr bool PACKS = MODE == MX_SCORES && FMT == MX_E2M3 && PARTS == MX_PARTS_SCORES && RESIDENT;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -531,29 +563,24 @@ mx4_product_kernel(const MxParams p) {
         for (int i = tid; i < quads * (QUAD / 16); i += THREADS) ((uint4*)smem)[i] = s[i];
     };
     __shared__ int s_bad;               // a bit per query to be scored in fp32 (packed here)
-    if (MODE == MX_SCORES && FMT == MX_E2M3 && RESIDENT && p.pack_here) {
+    if (PACKS && p.pack_here) {
         // very few queries: packing them in every workgroup is shorter than a launch before this one (times below MX_PACK_HERE)
         if (tid == 0) s_bad = 0;
         __syncthreads();
-        const int sub = tid & 7;
-        for (int i = tid >> 3; i < p.nq * p.nkq * 8; i += THREADS / 8) {
+        for (int i = tid; i < p.nq * p.nkq * 8; i += THREADS) {
             const int ql = i / (p.nkq * 8), b = i - ql * (p.nkq * 8);
+            MxBlock x = mx_load_block(p.q, p.q_dtype, (int64_t)ql * p.d + b * 32, p.d - b * 32);
             bool exact = false;
-            float x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int at = b * 32 + sub * 4 + e;
-                x[e] = at < p.d ? load_as_f32(p.q, p.q_dtype, (int64_t)ql * p.d + at) : 0.f;
-                exact |= !(fabsf(x[e]) < 0x1p63f);              // not finite, or its square may not be
-            }
-            mx_pack_lane(x, b, sub, PARTS, BQ, ql, (uint8_t*)smem);
+            for (int e = 0; e < 16; ++e) exact |= !(fabsf(x.even[e]) < 0x1p63f) || !(fabsf(x.odd[e]) < 0x1p63f);      // not finite, or its square may not be
+            mx_pack_block(x, b, PARTS, BQ, ql, (uint8_t*)smem);
             if (exact) atomicOr(&s_bad, 1 << ql);
         }
     } else if constexpr (RESIDENT) {
         stage(0, p.nkq);
     }
     __syncthreads();
-    if (MODE == MX_SCORES && FMT == MX_E2M3 && RESIDENT && p.pack_here) redo = s_bad;
+    if (PACKS && p.pack_here) redo = s_bad;
 
     const int64_t per_round = (int64_t)p.S * WAVES;
     const int64_t rounds = (p.ntiles + per_round - 1) / per_round;
