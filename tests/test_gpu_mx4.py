@@ -134,7 +134,7 @@ def test_numpy_rows_take_the_same_way(mx4):
     (4096, 768, 32, 1, 1), (4096, 768, 33, 100, 1), (5000, 768, 300, 100, 2),
     (20000, 100, 513, 100, 3), (9000, 17, 64, 512, 2), (9000, 48, 64, 1500, 1), (9000, 48, 130, 2048, 2),
     (777, 768, 1, 100, 1), (255, 16, 257, 5, 1), (257, 16, 256, 300, 1), (1, 8, 3, 4, 1), (33, 1, 2, 7, 33),
-    (16384, 64, 5, 10, 1), (16385, 64, 5, 10, 2),          # the border of the sampled floor
+    (16384, 64, 5, 10, 1), (16385, 64, 5, 10, 2),
     (3000, 1000, 40, 50, 1), (3000, 1536, 129, 20, 1),     # fewer queries per block: longer vectors
     (2000, 4096, 70, 30, 1), (1500, 8192, 3, 20, 1),       # the query block goes through LDS in turns
 ])
@@ -170,6 +170,27 @@ def test_search_equals_a_bf16_index_of_the_same_values(R, n, d, nq, k):
     assert np.array_equal(I, I2) and np.array_equal(D.view(np.uint32), D2.view(np.uint32))
     st = ix.last_bf16_stats()
     assert st["candidates"] >= k and st["exact_queries"] == 0
+
+
+@pytest.mark.parametrize("n,d,nq,k", [(4095, 64, 300, 229), (4097, 40, 257, 2048), (8191, 33, 9, 100), (8192, 33, 9, 100),
+                                      (8193, 320, 30, 229), (65537, 16, 3, 900), (3300, 512, 300, 2000), (2049, 100, 500, 3)])
+@pytest.mark.parametrize("kind", ["plain", "shifted", "few numbers", "one score"])
+def test_every_length_has_a_floor(R, n, d, nq, k, kind):
+    """Floors from samples of every size, from scores that all lie on one side of zero, that are few, or equal."""
+    X, Q = gaussian(n, (n, d)), gaussian(n + 1, (nq, d))
+    if kind == "shifted":
+        X[:, 0], Q[:, 0] = 40, np.where(np.arange(nq) % 2, 3, -3)
+    elif kind == "few numbers":
+        X[np.arange(n) % 41 != 7, 3 % d] = np.nan
+    elif kind == "one score":
+        X[:], Q[nq // 2] = X[0], 0
+    ix = index(R, X)
+    D, I = ix.search(Q, k)
+    some = np.unique(np.r_[0, nq // 2, nq - 1, np.random.default_rng(1).integers(0, nq, 6)])
+    assert_bits(D[some], I[some], Q[some], M.rounded(X), k)
+    ix.set_param("bf16_candidates", 128)
+    D2, I2 = ix.search(Q, k)
+    assert np.array_equal(I, I2) and np.array_equal(D.view(np.uint32), D2.view(np.uint32))
 
 
 def test_rows_in_groups_and_order_do_not_break_the_floor(R):
