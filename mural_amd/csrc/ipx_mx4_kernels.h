@@ -834,7 +834,7 @@ mx4_floor_kernel(const float* __restrict__ sample, int m, int j, int64_t N, floa
     __shared__ int s_need, s_bin;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t q = blockIdx.x;
-    // entries 4 tid .. + 3 of every 4096: ordered score bits, 0 for what is never a hit (NaN, -inf) and from entry m on
+    // entries 4 tid .. + 3 of every 4096: ordered score bits, 0 for what is never a hit (NaN, -inf) and from entry m on (fewer than M only of short indexes)
     uint32_t v[PER];
     uint32_t best = 0;
 #pragma unroll
@@ -843,7 +843,7 @@ mx4_floor_kernel(const float* __restrict__ sample, int m, int j, int64_t N, floa
         const float s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            v[i + e] = s[e] > -FLT_MAX && i * 1024 + tid * 4 + e < m ? f32_ordered(s[e]) : 0u;
+            v[i + e] = s[e] > -FLT_MAX && (PER > 4 || i * 1024 + tid * 4 + e < m) ? f32_ordered(s[e]) : 0u;
             best = max(best, v[i + e]);
         }
     }
