@@ -122,7 +122,7 @@ __device__ __forceinline__ uint32_t div_by(uint32_t i, uint64_t magic) {      //
 // ---- quantisation ----------------------------------------------------------------------------------------------
 // Rows [n, d] (f32 / f16 / bf16, `stride` elements apart) -> codes and scales, in the external form or (INDEX) at rows
 // row0.. of an index. Four adjacent lanes per block, eight elements each: the block's largest magnitude is two exchanges of
-// lanes away. Bound by HBM.
+// lanes away. Bound by HBM: 500k x 768 f16 in 190 us (0.97 GB at 5.1 TB/s).
 template <bool INDEX>
 __global__ void __launch_bounds__(256)
 mx4_quantize_kernel(const void* __restrict__ src, int dtype, int64_t stride, uint32_t total, uint64_t magic, int np, int d,
@@ -195,7 +195,7 @@ mx4_place_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ 
     Xs[mx_scale_at(row0 + r, b, nkq)] = scales[gid];
 }
 
-// external form -> values
+// external form -> values; bound by its stores: 500k x 768 to fp32 in 325-355 us (1.74 GB at 5.1 TB/s)
 __global__ void __launch_bounds__(256)
 mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t total, uint64_t magic, int np,
                       int d, int nb, void* __restrict__ out, int dtype) {
@@ -213,7 +213,7 @@ mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
 // max |x|^2 over rows [row0, row0 + n) of an mx4 index, for the margin rule (rescore_kernel), as float bits. A row with a
 // NaN block scores NaN in the scan and in the exact chain alike — it is never a candidate and never a result — so it does
 // not enter the maximum; a sum that overflows does (as inf: every margin test then fails, which is intended).
-// One wave per group of 32 rows: the loads of the scan.
+// One wave per group of 32 rows: the loads of the scan (1.8M x 768 in 235 us, once per row; quantising them from fp32 takes 1.2 ms).
 __global__ void __launch_bounds__(256)
 mx4_norm_max_kernel(const uint8_t* __restrict__ X, const uint8_t* __restrict__ Xs, int64_t row0, int64_t n, int nks, int nkq,
                     uint32_t* __restrict__ maxsq) {
@@ -248,8 +248,8 @@ mx4_norm_max_kernel(const uint8_t* __restrict__ X, const uint8_t* __restrict__ X
 // The product is rounded to fp32, then once to the output type. The empty slot id -1 gives a row of zeros; so does any other
 // id outside the index, which also sets *err. A row has 2^l2 adjacent lanes, each with several pieces of eight elements (the
 // host leaves the fewest lanes idle: lookup_lanes): a row's address takes two dependent loads, one piece per lane was bound
-// by them (698k rows of 768 out of 1.8M, bf16 out: 480 us; so 366). Rows are gathered in 64-byte pieces, for which the
-// memory moves 128 bytes: 0.9 KB per mx4 row of 768 elements, that and the output at 4.6 TB/s.
+// by them (698k rows of 768 out of 1.8M, bf16 out: 480 us; so 366). Bound by the gather, 64-byte pieces and a scale line per
+// row: 0.67 GB read (0.28 GB are asked for) and 1.07 GB written, 4.7 TB/s.
 template <int XFMT>
 __global__ void __launch_bounds__(256)
 lookup_kernel(const void* __restrict__ X, const uint8_t* __restrict__ Xs, int nks, int nkq, int64_t id_base, int64_t N,
@@ -516,6 +516,11 @@ __device__ __forceinline__ void static_for(F&& f) {
 // MX_SCORES: queries are the A operand, so that a lane holds one row and a store instruction writes two lines of 32
 // consecutive columns (with rows as A: 32 pieces of 32 bytes, one query each; 8192 x 32768 scores took 500 us so).
 // MX_SEARCH: rows are the A operand: a lane holds 16 rows of one query and its floor.
+// What bounds it: a search of one query the rows (1.8M x 768: 116 us, 6.3 TB/s); scores of mx4 queries their stores (8192 x
+// 32768: 235 us, 4.6 TB/s); scores of 1000 fp32 queries x 100k x 768 (198 us, 3.9 PFLOP/s over the five parts) and a search of
+// 1000 x 500k x 768 (407 us, 3.8 PFLOP/s over the two) the matrix cores and the chip's power: they are busy in 0.64 and
+// 0.49 of the cycles, at 1.5 and 1.9 GHz. Of the search's 407 us 50 are the hits' stores, behind which a wave waits for its
+// row loads (no hits: 350 us; testing four rows at a time for hits, 388 us of 394; a mask and a loop over its bits, 525).
 template <int CG, int RG, int WAVES, int PARTS, int FMT, int MODE, bool RESIDENT>
 __global__ void __launch_bounds__(WAVES * 64)
 mx4_product_kernel(const MxParams p) {
@@ -939,6 +944,7 @@ mx4_floor_kernel(const float* __restrict__ sample, int m, int j, int64_t N, floa
 
 // ---- the hits of one query -> its best kc, sorted --------------------------------------------------------------
 // lists: [nq][nlists][cap] hits in any order, cnt[q * nlists + l] of them. One workgroup of 1024 per query, nlists <= 8192.
+// (7 us for one query, 24 us for 1000 queries of 1250 out of some 2500 hits: latency.)
 // Little more hits than wanted is the rule (mx4_floor_kernel). A histogram of the scores between the lowest and the best
 // hit, linear in the bits, finds the step that holds the kc-th; the hits from that step up go to their step's place in LDS
 // (Pmax slots), where each counts the better ones of its own step: its place in the list, no sort. Should they be more than
