@@ -519,8 +519,8 @@ __device__ __forceinline__ void static_for(F&& f) {
 // What bounds it: a search of one query the rows (1.8M x 768: 116 us, 6.3 TB/s); scores of mx4 queries their stores (8192 x
 // 32768: 235 us, 4.6 TB/s); scores of 1000 fp32 queries x 100k x 768 (198 us, 3.9 PFLOP/s over the five parts) and a search of
 // 1000 x 500k x 768 (407 us, 3.8 PFLOP/s over the two) the matrix cores and the chip's power: they are busy in 0.64 and
-// 0.49 of the cycles, at 1.5 and 1.9 GHz. Of the search's 407 us 50 are the hits' stores, behind which a wave waits for its
-// row loads (no hits: 350 us; testing four rows at a time for hits, 388 us of 394; a mask and a loop over its bits, 525).
+// 0.49 of the cycles, at 1.5 and 1.9 GHz. Of the search's 407 us 50 are its hits (none: 350 us). Testing four rows at a time
+// for them takes 388 us of 394, holding them in LDS and writing them together 460 of 425, a mask and a loop over its bits 665.
 template <int CG, int RG, int WAVES, int PARTS, int FMT, int MODE, bool RESIDENT>
 __global__ void __launch_bounds__(WAVES * 64)
 mx4_product_kernel(const MxParams p) {
