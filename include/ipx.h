@@ -180,7 +180,7 @@ int ipx_add_mx4(ipx_index* idx, const uint8_t* codes, const uint8_t* scales, int
 /* out[i][j] = <q_i, row row0 + j of the index>, fp32 [nq, n], storage 3 only. q: [nq, d] of q_dtype, taken to within 2^-20
  * of the largest magnitude of each block of 32 elements (in practice 2^-24), products and sums in fp32; a query with a
  * NaN or an infinity is multiplied element by element. ipx_scores_mx4: queries in mx4, products exact.
- * n < 2^27. With on_device != 0 stream-ordered: never synchronises, and allocates only where more than 4 queries are the
+ * n < 2^27. With on_device != 0 stream-ordered: never synchronises, and allocates only where more than 32 queries are the
  * most so far (the index's query buffers).
  * HIP graphs: run a call of the size once, then capture it (on_device != 0; ipx_lookup likewise). A replay counts as a call
  * on the index (one at a time) and reads the rows as the index held them when it was captured; adding rows, or larger

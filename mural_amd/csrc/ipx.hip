@@ -1382,10 +1382,10 @@ int scan_bf16_path(ipx_index* ix, const float* dq, const float* dw, int A, int l
 // ---- mx4 rows (storage 3) -------------------------------------------------------------------------------------
 using ipx::MX_PARTS_SCORES;
 using ipx::MX_PARTS_SEARCH;
-// ipx_scores: up to this many queries are packed by the product kernel itself, in every workgroup, not by a kernel before it
-// (with it -> without, us; 1 query: 1000 x 768 rows 13.9 -> 9.4, 100k 17.3 -> 15.0, 1M 90 -> 91; 4 queries: 13.8 -> 10.9,
-// 17.3 -> 16.1, 97 -> 96.5; 8 queries: 13.9 -> 12.9, 17.9 -> 18.3, 103 -> 108)
-constexpr int MX_PACK_HERE = 4;
+// ipx_scores: up to this many queries (one block) are packed by the product kernel itself, in every workgroup, not by a kernel
+// before it. With it <- without, us: 8 queries x 1000 x 768 rows 10.4 <- 14.4, x 100k 15.3 <- 18.8, x 1M 105 <- 106; 32 queries:
+// 12.6 <- 13.8, 19.2 <- 20.1, 120 <- 121; 1 query x 1000 rows 10.2.
+constexpr int MX_PACK_HERE = 32;
 constexpr int64_t MX_SCORES_SLICE = 1 << 18;      // queries per pass of ipx_scores: bounds the workspace (4 KB a query of 768) and a launch's threads
 constexpr int MX_MAX_K = IPX_MAX_K;      // deepest list of a search
 constexpr int MX_SLICE = 4096;           // queries per pass of a search (bounds the workspace)

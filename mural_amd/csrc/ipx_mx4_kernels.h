@@ -569,7 +569,7 @@ mx4_product_kernel(const MxParams p) {
     };
     __shared__ int s_bad;               // a bit per query to be scored in fp32 (packed here)
     if (PACKS && p.pack_here) {
-        // very few queries: packing them in every workgroup is shorter than a launch before this one (times below MX_PACK_HERE)
+        // few queries: packing them in every workgroup is shorter than a launch before this one (MX_PACK_HERE)
         if (tid == 0) s_bad = 0;
         __syncthreads();
         for (int i = tid; i < p.nq * p.nkq * 8; i += THREADS) {

@@ -442,7 +442,7 @@ def test_a_graph_outlives_larger_calls_and_added_rows(R, mx4, torch, storage):
     X = torch.from_numpy(gaussian(101, (1500, 96))).cuda()
     ix = R.FlatIPIndex(96, storage=storage)
     ix.add(X)
-    q = torch.from_numpy(gaussian(102, (9, 96))).cuda()
+    q = torch.from_numpy(gaussian(102, (39, 96))).cuda()
     codes, scales = mx4.quantize(q)
     ids = torch.arange(1499, -1, -3, device="cuda")
 
@@ -468,13 +468,13 @@ def test_a_graph_outlives_larger_calls_and_added_rows(R, mx4, torch, storage):
 
 
 def test_scores_of_a_query_do_not_depend_on_the_others(R, torch):
-    """Up to four queries are packed by the product kernel, more by a kernel before it: the same bits."""
+    """Up to 32 queries are packed by the product kernel, more by a kernel before it: the same bits."""
     X, q = gaussian(105, (700, 300)), gaussian(106, (40, 300))
     q[1, 7], q[2, 299], q[3] = np.inf, np.nan, q[3] * np.float32(2.0 ** 100)
     ix = index(R, X)
     tq = torch.from_numpy(q).cuda()
     full = ix.scores(tq).cpu().numpy()
-    for n in (1, 2, 3, 4, 5, 33):
+    for n in (1, 2, 3, 4, 5, 32, 33):
         for lo in (0, 1, 7):
             assert np.array_equal(ix.scores(tq[lo:lo + n]).cpu().numpy(), full[lo:lo + n], equal_nan=True)
 
