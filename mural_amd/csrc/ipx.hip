@@ -1463,10 +1463,10 @@ float mx4_acc_coef(int d, int nks, int parts) { return (float)((d + 1 + 4.0 * (n
 
 // fp32 (f16, bf16) queries -> parts, their norms, `todo` cleared
 int launch_mx4_pack(ipx_index* ix, const void* q, int dtype, int64_t nq, int parts, int bq, ipx::MxQueryInfo* info, int* todo, hipStream_t st) {
-    int l2 = 3;
-    while (l2 < 6 && (1 << l2) < ix->nkq_x * 8) ++l2;
+    int l2 = 1;
+    while (l2 < 6 && (1 << l2) < ix->nks_x * 2) ++l2;
     hipLaunchKernelGGL(ipx::mx4_pack_queries_kernel, dim3((unsigned)(((nq << l2) + 255) / 256)), dim3(256), 0, st, q, dtype, (int)nq, ix->d, parts,
-                       bq, ix->nkq_x, l2, (uint8_t*)ix->Qp.p, info, todo);
+                       bq, ix->nks_x, ix->nkq_x, l2, (uint8_t*)ix->Qp.p, info, todo);
     IPX_HIP(hipGetLastError());
     return 0;
 }
@@ -1705,9 +1705,9 @@ int scores_slice(ipx_index* ix, const void* dq, int q_dtype, const uint8_t* q_sc
         const MxGeom g = mx4_geometry(ix, nq, quad1, ipx::MX_SCORES, groups);
         p.gstep = g.rg;
         if (int rc = ix->Qp.ensure((size_t)g.nqb * ix->nkq_x * quad1 * g.cg)) return rc;
-        const int64_t total = nq * ix->nkq_x * 8;
+        const int64_t total = nq * ix->nks_x * 2;
         hipLaunchKernelGGL(ipx::mx4_pack_codes_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, (const uint8_t*)dq,
-                           q_scales, ix->d, 32 * g.cg, ix->nkq_x, total, (uint8_t*)ix->Qp.p);
+                           q_scales, ix->d, 32 * g.cg, ix->nks_x, ix->nkq_x, total, (uint8_t*)ix->Qp.p);
         IPX_HIP(hipGetLastError());
         ix->Qp.captured |= captured;
         p.Q = (const uint8_t*)ix->Qp.p;

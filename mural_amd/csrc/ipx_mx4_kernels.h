@@ -394,11 +394,11 @@ __device__ __forceinline__ void mx_pack_block(MxBlock& x, int b, int parts, int 
     }
 }
 
-// A lane per block; 2^l2 lanes (8 to 64) per query. Neighbouring queries write neighbouring 16-byte pieces: they share a
+// A lane per block, blocks up to whole K-sets (the rest of the last quad is not multiplied); 2^l2 lanes (2 to 64) per query. Neighbouring queries write neighbouring 16-byte pieces: they share a
 // workgroup, and an XCD. 3813 queries of 576 in 5 parts: 17 us; four elements a lane,
 // converted by ordinary arithmetic, took 24.
 __global__ void __launch_bounds__(256)
-mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, int parts, int bq, int nkq, int l2,
+mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, int parts, int bq, int nks, int nkq, int l2,
                         uint8_t* __restrict__ dst, MxQueryInfo* __restrict__ info, int* __restrict__ todo) {
     const int64_t q = ((int64_t)xcd_remap(blockIdx.x, gridDim.x) * 256 + threadIdx.x) >> l2;
     if (q >= nq) return;
@@ -406,7 +406,7 @@ mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, 
     const int lanes = 1 << l2, first = threadIdx.x & (lanes - 1), ql = (int)(q % bq);
     int nonzero = 0;
     float ss = 0.f, rr = 0.f;
-    for (int b = first; b < nkq * 8; b += lanes) {
+    for (int b = first; b < nks * 2; b += lanes) {
         MxBlock x = mx_load_block(src, dtype, q * (int64_t)d + b * 32, d - b * 32);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -429,14 +429,14 @@ mx4_pack_queries_kernel(const void* __restrict__ src, int dtype, int nq, int d, 
     }
 }
 
-// external mx4 rows as queries (one part, E2M1); one thread per block of every query, blocks up to whole quads
+// external mx4 rows as queries (one part, E2M1); one thread per block of every query, blocks up to whole K-sets
 __global__ void __launch_bounds__(256)
-mx4_pack_codes_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int d, int bq, int nkq,
+mx4_pack_codes_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int d, int bq, int nks, int nkq,
                       int64_t total, uint8_t* __restrict__ dst) {
     const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (gid >= total) return;
-    const int64_t q = gid / (nkq * 8);
-    const int b = (int)(gid - q * (nkq * 8)), nb = (d + 31) / 32;
+    const int64_t q = gid / (nks * 2);
+    const int b = (int)(gid - q * (nks * 2)), nb = (d + 31) / 32;
     uint32_t w[4] = {0, 0, 0, 0};
     uint8_t sc = 0;
     if (b < nb) {
@@ -560,8 +560,8 @@ mx4_product_kernel(const MxParams p) {
             redo |= q < p.nq && !(p.info[q].sumsq <= FLT_MAX) ? 1 : 0;
         }
     }
-    // (the packing kernels do not write the places of queries behind the last one: what lies there only reaches sums that are
-    // never stored)
+    // (the packing kernels do not write the places of queries behind the last one, whose sums are never stored, nor those of
+    // K-sets behind the last one, which are not multiplied)
     auto stage = [&](int quad0, int quads) {
         const uint4* s = (const uint4*)(qblock + (size_t)quad0 * QUAD);
 #pragma unroll 4
@@ -572,8 +572,8 @@ mx4_product_kernel(const MxParams p) {
         // few queries: packing them in every workgroup is shorter than a launch before this one (MX_PACK_HERE)
         if (tid == 0) s_bad = 0;
         __syncthreads();
-        for (int i = tid; i < p.nq * p.nkq * 8; i += THREADS) {
-            const int ql = i / (p.nkq * 8), b = i - ql * (p.nkq * 8);
+        for (int i = tid; i < p.nq * p.nks * 2; i += THREADS) {
+            const int ql = i / (p.nks * 2), b = i - ql * (p.nks * 2);
             MxBlock x = mx_load_block(p.q, p.q_dtype, (int64_t)ql * p.d + b * 32, p.d - b * 32);
             bool exact = false;
 #pragma unroll
